@@ -168,6 +168,103 @@ int b200fa_key_blocks_host(const b200fa_problem* problem, int32_t seq, int32_t m
 int b200fa_query_blocks_host(const b200fa_problem* problem, int32_t seq, int32_t c0, int32_t c1, int32_t* out,
                              int32_t max_blocks);
 
+/* ---- Paged key-value cache (no counterpart in the reference).
+ * A cache tensor is (num_pages, page_size, heads_kv, head_dim) BF16; key j of sequence b is row j % page_size of page
+ * block_table[b][j / page_size]. A table entry outside [0, num_pages) holds no page: its positions are not visible, and
+ * nothing is written there. Lengths outside [0, max_pages * page_size] are cut to that range. The integer tensors are
+ * int32 with contiguous columns. */
+
+/* Attention of one new token per sequence over the cache: out = softmax(scale q k^T) v over the keys that the token, the
+ * last of the cache_seqlens[b] keys of its sequence, sees: the last window_left + 1 of them (-1 = all) and the first
+ * sink_size. A sequence that sees no key gets zeros and a log-sum-exp of -inf.
+ * Strides in elements: q and out [0] sequence, [1] head; caches [0] page, [1] row, [2] head. */
+typedef struct b200fa_paged_args {
+  int32_t batch, heads_q, heads_kv, head_dim;
+  int32_t num_pages, page_size, max_pages; /* max_pages: columns of block_table */
+  int32_t window_left, sink_size;
+  float softmax_scale;
+  const void* q;                /* (batch, heads_q, head_dim) */
+  const void* k_cache;
+  const void* v_cache;
+  const int32_t* block_table;   /* (batch, max_pages), row stride table_stride */
+  const int32_t* cache_seqlens; /* (batch) keys per sequence, the new token's among them */
+  void* out;                    /* bf16, shape of q */
+  float* softmax_lse;           /* fp32 (batch, heads_q) contiguous; natural log */
+  int64_t q_stride[2], k_stride[3], v_stride[3], out_stride[2], table_stride;
+  void* workspace;
+  size_t workspace_bytes;
+} b200fa_paged_args;
+
+/* A function of batch, heads_q, heads_kv, head_dim, page_size and max_pages alone. */
+size_t b200fa_paged_decode_workspace_bytes(const b200fa_paged_args* args);
+int b200fa_paged_decode(const b200fa_paged_args* args, void* stream);
+/* Host twin of the key selection: the keys that the new token of a sequence of `length` keys sees, `capacity` being
+ * max_pages * page_size, in the order in which the kernel walks them. Returns their number. */
+int b200fa_paged_keys_host(int32_t length, int32_t capacity, int32_t window_left, int32_t sink_size, int32_t* keys,
+                           int32_t max_keys);
+
+typedef struct b200fa_kv_cache {
+  int32_t num_pages, page_size, heads_kv, head_dim; /* head_dim: a multiple of 8 of at most 1024 */
+  void* k_cache;
+  void* v_cache;
+  int64_t k_stride[3], v_stride[3]; /* [0] page, [1] row, [2] head */
+} b200fa_kv_cache;
+
+/* Writes the keys and values of new tokens into the pages: token i of sequence b becomes key cache_seqlens[b] + i.
+ * Fixed length: k, v (batch, rows, heads_kv, head_dim), cu_seqlens NULL. Packed: k, v (rows, heads_kv, head_dim),
+ * cu_seqlens (batch + 1); rows behind the last sequence are left out. No two sequences may write to the same page. */
+typedef struct b200fa_append_args {
+  b200fa_kv_cache cache;
+  const void* k;
+  const void* v;
+  int64_t k_stride[3], v_stride[3]; /* [0] sequence, [1] row, [2] head */
+  int64_t rows;
+  const int32_t* cu_seqlens;
+  const int32_t* cache_seqlens; /* (batch) keys held before the call */
+  const int32_t* block_table;   /* (batch, max_pages) */
+  int64_t table_stride;
+  int32_t batch, max_pages;
+} b200fa_append_args;
+int b200fa_append_kv(const b200fa_append_args* args, void* stream);
+
+/* Copies page source_pages[i] of both caches to page target_pages[i], for i < count; a pair with an entry outside
+ * [0, num_pages) is skipped. The targets must differ from one another and from every source. */
+int b200fa_copy_pages(const b200fa_kv_cache* cache, const int32_t* source_pages, const int32_t* target_pages, int32_t count,
+                      void* stream);
+
+/* Which sequence holds which page. page_refs (num_pages) counts the table entries that name a page; a page with a count
+ * <= 0 is free. The calls read block_table and page_refs and write new ones, which must not overlap them; an entry that
+ * holds no page comes out as -1. Pages are handed out lowest first, requests served in the order (sequence, entry); when
+ * the free pages run out, the entries that got none are -1. */
+typedef struct b200fa_pages_args {
+  int32_t sequences, rows; /* rows of block_table and of block_table_out */
+  int32_t max_pages, num_pages, page_size;
+  const int32_t* block_table; /* (sequences, max_pages), row stride table_stride */
+  int64_t table_stride;
+  const int32_t* page_refs;     /* (num_pages) */
+  const int32_t* cache_seqlens; /* (sequences) */
+  int32_t* block_table_out;     /* (rows, max_pages) contiguous */
+  int32_t* page_refs_out;       /* (num_pages) */
+  int32_t* source_pages;        /* pairs for b200fa_copy_pages, -1 = none: (rows) for a fork, (num_pages / 2) for compacting */
+  int32_t* target_pages;
+  void* workspace; /* b200fa_pages_workspace_bytes(num_pages); not needed by b200fa_free_pages */
+  size_t workspace_bytes;
+} b200fa_pages_args;
+size_t b200fa_pages_workspace_bytes(int32_t num_pages);
+/* Pages for the next new_tokens[b] tokens of every sequence: the entries behind the ceil(cache_seqlens[b] / page_size)
+ * first ones that lack a page get a free one. */
+int b200fa_reserve_pages(const b200fa_pages_args* args, const int32_t* new_tokens, void* stream);
+/* Row i of block_table_out becomes a continuation of sequence parents[i]: it shares the parent's full pages and gets a
+ * page of its own for the partly filled last one, to be copied (source_pages[i], target_pages[i]). child_seqlens[i] is
+ * the parent's length; a parent outside [0, sequences) gives an empty row. */
+int b200fa_fork_pages(const b200fa_pages_args* args, const int32_t* parents, int32_t* child_seqlens, void* stream);
+/* Gives the entries [first_entry[b], last_entry[b]) of every sequence back: each becomes -1 and its page loses a
+ * reference. */
+int b200fa_free_pages(const b200fa_pages_args* args, const int32_t* first_entry, const int32_t* last_entry, void* stream);
+/* Moves the pages in use to the front of the pool: with n of them, the i-th one at or behind n goes to the i-th free page
+ * in front of n. Tables and counts follow, and the pairs (source_pages, target_pages) say what to copy. */
+int b200fa_compact_pages(const b200fa_pages_args* args, void* stream);
+
 /* Reads and clears the device-side status word (synchronises the device). 0 = no kernel wait ran out of time. */
 int b200fa_device_status(void);
 const char* b200fa_last_error(void);

@@ -32,6 +32,16 @@ EXPORTS = (
     "b200fa_interseq_metadata_host",
     "b200fa_key_blocks_host",
     "b200fa_query_blocks_host",
+    "b200fa_paged_decode_workspace_bytes",
+    "b200fa_paged_decode",
+    "b200fa_paged_keys_host",
+    "b200fa_append_kv",
+    "b200fa_copy_pages",
+    "b200fa_pages_workspace_bytes",
+    "b200fa_reserve_pages",
+    "b200fa_fork_pages",
+    "b200fa_free_pages",
+    "b200fa_compact_pages",
     "b200fa_device_status",
     "b200fa_last_error",
     "b200fa_version",
@@ -110,6 +120,61 @@ class BwdArgs(ctypes.Structure):
     ]
 
 
+class PagedArgs(ctypes.Structure):
+    _fields_ = [
+        *((name, ctypes.c_int32) for name in ("batch", "heads_q", "heads_kv", "head_dim", "num_pages", "page_size",
+                                              "max_pages", "window_left", "sink_size")),
+        ("softmax_scale", ctypes.c_float),
+        *((name, ctypes.c_void_p) for name in ("q", "k_cache", "v_cache", "block_table", "cache_seqlens", "out",
+                                               "softmax_lse")),
+        ("q_stride", Stride2),
+        ("k_stride", Stride3),
+        ("v_stride", Stride3),
+        ("out_stride", Stride2),
+        ("table_stride", ctypes.c_int64),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
+class KvCache(ctypes.Structure):
+    _fields_ = [
+        *((name, ctypes.c_int32) for name in ("num_pages", "page_size", "heads_kv", "head_dim")),
+        ("k_cache", ctypes.c_void_p),
+        ("v_cache", ctypes.c_void_p),
+        ("k_stride", Stride3),
+        ("v_stride", Stride3),
+    ]
+
+
+class AppendArgs(ctypes.Structure):
+    _fields_ = [
+        ("cache", KvCache),
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("k_stride", Stride3),
+        ("v_stride", Stride3),
+        ("rows", ctypes.c_int64),
+        ("cu_seqlens", ctypes.c_void_p),
+        ("cache_seqlens", ctypes.c_void_p),
+        ("block_table", ctypes.c_void_p),
+        ("table_stride", ctypes.c_int64),
+        ("batch", ctypes.c_int32),
+        ("max_pages", ctypes.c_int32),
+    ]
+
+
+class PagesArgs(ctypes.Structure):
+    _fields_ = [
+        *((name, ctypes.c_int32) for name in ("sequences", "rows", "max_pages", "num_pages", "page_size")),
+        ("block_table", ctypes.c_void_p),
+        ("table_stride", ctypes.c_int64),
+        *((name, ctypes.c_void_p) for name in ("page_refs", "cache_seqlens", "block_table_out", "page_refs_out",
+                                               "source_pages", "target_pages", "workspace")),
+        ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
 class LibraryError(RuntimeError):
     pass
 
@@ -151,6 +216,22 @@ def library() -> ctypes.CDLL:
     lib.b200fa_key_blocks_host.argtypes = [ctypes.POINTER(Problem)] + [ctypes.c_int32] * 3 + [ctypes.c_void_p, ctypes.c_int32]
     lib.b200fa_query_blocks_host.restype = ctypes.c_int
     lib.b200fa_query_blocks_host.argtypes = [ctypes.POINTER(Problem)] + [ctypes.c_int32] * 3 + [ctypes.c_void_p, ctypes.c_int32]
+    lib.b200fa_paged_decode_workspace_bytes.restype = ctypes.c_size_t
+    lib.b200fa_paged_decode_workspace_bytes.argtypes = [ctypes.POINTER(PagedArgs)]
+    lib.b200fa_paged_decode.restype = ctypes.c_int
+    lib.b200fa_paged_decode.argtypes = [ctypes.POINTER(PagedArgs), ctypes.c_void_p]
+    lib.b200fa_paged_keys_host.restype = ctypes.c_int
+    lib.b200fa_paged_keys_host.argtypes = [ctypes.c_int32] * 4 + [ctypes.c_void_p, ctypes.c_int32]
+    lib.b200fa_append_kv.restype = ctypes.c_int
+    lib.b200fa_append_kv.argtypes = [ctypes.POINTER(AppendArgs), ctypes.c_void_p]
+    lib.b200fa_copy_pages.restype = ctypes.c_int
+    lib.b200fa_copy_pages.argtypes = [ctypes.POINTER(KvCache), ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int32, ctypes.c_void_p]
+    lib.b200fa_pages_workspace_bytes.restype = ctypes.c_size_t
+    lib.b200fa_pages_workspace_bytes.argtypes = [ctypes.c_int32]
+    for name, extra in (("reserve", 1), ("fork", 2), ("free", 2), ("compact", 0)):
+        function = getattr(lib, f"b200fa_{name}_pages")
+        function.restype = ctypes.c_int
+        function.argtypes = [ctypes.POINTER(PagesArgs)] + [ctypes.c_void_p] * (extra + 1)
     lib.b200fa_device_status.restype = ctypes.c_int
     lib.b200fa_device_status.argtypes = []
     lib.b200fa_last_error.restype = ctypes.c_char_p

@@ -116,14 +116,110 @@ def prepare_inter_sequence_metadata(
     return ops.prepare_inter_sequence_metadata(cu_seqlens_q, cu_seqlens_k, visibility_bits)
 
 
+def flash_attn_paged_func(
+    q: Tensor, k_cache: Tensor, v_cache: Tensor, block_table: Tensor, cache_seqlens: Tensor,
+    softmax_scale: float | None = None, window_size: tuple[int, int] = (-1, -1), sink_size: int = 0,
+    return_attn_probs: bool = False,
+) -> Tensor | tuple[Tensor, Tensor]:
+    """Attention of one new token per sequence over a paged key-value cache (inference only).
+
+    q (sequences, heads_q, head_dim); k_cache, v_cache (pages, page_size, heads_kv, head_dim), any strides the kernels can
+    read; block_table (sequences, max_pages) int32, the page of every page_size keys, where an entry outside the cache
+    holds no keys; cache_seqlens (sequences) int32, the keys of each sequence with those of the new token, which is the
+    last one. It sees the last window_size[0] + 1 keys (-1: all) and the first `sink_size`; window_size[1] has no effect.
+    A sequence without visible keys gets zeros and a log-sum-exp of -inf. Returns out, and with `return_attn_probs`
+    (out, softmax_lse), softmax_lse (sequences, heads_q) float32."""
+    from ._impl import paged
+
+    return paged.flash_attn_paged(q, k_cache, v_cache, block_table, cache_seqlens, softmax_scale, window_size, sink_size, return_attn_probs)
+
+
+def append_paged_kv(
+    k: Tensor, v: Tensor, k_cache: Tensor, v_cache: Tensor, block_table: Tensor, cache_seqlens: Tensor,
+    cu_seqlens: Tensor | None = None,
+) -> None:
+    """Writes the keys and values of new tokens into the pages of their sequences, in place.
+
+    k, v (sequences, tokens, heads_kv, head_dim), or packed (total, heads_kv, head_dim) with cu_seqlens (sequences + 1);
+    token i of sequence b becomes key cache_seqlens[b] + i, so cache_seqlens counts the keys held before the call. Tokens
+    whose table entry holds no page are dropped. Sequences must not share the pages that are written to."""
+    from ._impl import paged  # noqa: F401  registers the op
+    import torch
+
+    torch.ops.zigfa.append_kv(k, v, k_cache, v_cache, block_table, cache_seqlens, cu_seqlens)
+
+
+def copy_kv_pages(k_cache: Tensor, v_cache: Tensor, source_pages: Tensor, target_pages: Tensor) -> None:
+    """Copies page source_pages[i] of both caches to page target_pages[i], in place; a pair with an entry outside the cache
+    (-1) is skipped. The targets must differ from one another and from every source."""
+    from ._impl import paged  # noqa: F401
+    import torch
+
+    torch.ops.zigfa.copy_pages(k_cache, v_cache, source_pages, target_pages)
+
+
+def reserve_kv_pages(
+    block_table: Tensor, cache_seqlens: Tensor, new_tokens: Tensor, page_refs: Tensor, page_size: int,
+) -> tuple[Tensor, Tensor]:
+    """Pages for the next new_tokens[b] tokens of every sequence: the table entries behind those that cache_seqlens[b]
+    tokens fill get a free page (page_refs <= 0) where they hold none, lowest pages first, in the order (sequence, entry);
+    -1 stays where no page is left. Returns the new (block_table, page_refs)."""
+    from ._impl import paged  # noqa: F401
+    import torch
+
+    return torch.ops.zigfa.reserve_pages(block_table, cache_seqlens, new_tokens, page_refs, page_size)
+
+
+def fork_kv_pages(
+    block_table: Tensor, cache_seqlens: Tensor, page_refs: Tensor, parents: Tensor, page_size: int,
+) -> tuple[Tensor, Tensor, Tensor, Tensor, Tensor]:
+    """New sequences that continue those named by `parents` (children) int32. A child shares its parent's full pages,
+    whose page_refs count it, and gets a free page for the partly filled last one, to be copied in every layer with
+    copy_kv_pages. Returns (child_table, child_seqlens, page_refs, source_pages, target_pages); a pair is -1 where nothing
+    has to be copied or no page was left (the child's table entry is then -1 too)."""
+    from ._impl import paged  # noqa: F401
+    import torch
+
+    return torch.ops.zigfa.fork_pages(block_table, cache_seqlens, page_refs, parents, page_size)
+
+
+def free_kv_pages(
+    block_table: Tensor, page_refs: Tensor, first_entry: Tensor, last_entry: Tensor,
+) -> tuple[Tensor, Tensor]:
+    """Gives the table entries [first_entry[b], last_entry[b]) of every sequence back: they become -1 and their pages lose
+    a reference each; a page without references is free. Whole sequences (0 to max_pages) and pages that a window has left
+    go the same way. Returns the new (block_table, page_refs)."""
+    from ._impl import paged  # noqa: F401
+    import torch
+
+    return torch.ops.zigfa.free_pages(block_table, page_refs, first_entry, last_entry)
+
+
+def compact_kv_pages(block_table: Tensor, page_refs: Tensor) -> tuple[Tensor, Tensor, Tensor, Tensor]:
+    """Moves the pages in use to the front of the pool: with n of them, the i-th page in use at or behind n goes to the
+    i-th free page in front of n. Returns the new (block_table, page_refs) and the pairs (source_pages, target_pages),
+    -1 behind the last one, to be copied in every layer with copy_kv_pages."""
+    from ._impl import paged  # noqa: F401
+    import torch
+
+    return torch.ops.zigfa.compact_pages(block_table, page_refs)
+
+
 __all__ = [
     "InterSequenceMetadata",
+    "append_paged_kv",
+    "compact_kv_pages",
+    "copy_kv_pages",
     "flash_attn_func",
     "flash_attn_inter_sequence_func",
     "flash_attn_inter_sequence_kvpacked_func",
     "flash_attn_kvpacked_func",
+    "flash_attn_paged_func",
     "flash_attn_qkvpacked_func",
     "flash_attn_varlen_func",
     "flash_attn_varlen_kvpacked_func",
+    "fork_kv_pages",
+    "free_kv_pages",
     "prepare_inter_sequence_metadata",
+    "reserve_kv_pages",
 ]
