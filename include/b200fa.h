@@ -168,6 +168,20 @@ int b200fa_key_blocks_host(const b200fa_problem* problem, int32_t seq, int32_t m
 int b200fa_query_blocks_host(const b200fa_problem* problem, int32_t seq, int32_t c0, int32_t c1, int32_t* out,
                              int32_t max_blocks);
 
+/* ---- Sliding window with sinks (no counterpart in the reference): b200fa_fwd and b200fa_bwd with the first sink_size
+ * keys of every sequence visible to each query row that the right bound lets see them, in front of the window. Without a
+ * left bound sink_size has no effect. Not for inter-sequence batches; head_dim 64, 72, 96, 128; softmax_scale > 0. In a packed batch, what
+ * stands in rows behind the last sequence, NaN included, has no effect on any result. */
+size_t b200fa_sink_fwd_workspace_bytes(const b200fa_problem* problem, int32_t sink_size);
+int b200fa_sink_fwd(const b200fa_fwd_args* args, int32_t sink_size, void* stream);
+size_t b200fa_sink_bwd_workspace_bytes(const b200fa_problem* problem, int32_t sink_size);
+int b200fa_sink_bwd(const b200fa_bwd_args* args, int32_t sink_size, void* stream);
+/* b200fa_key_blocks_host and b200fa_query_blocks_host with sinks. */
+int b200fa_sink_key_blocks_host(const b200fa_problem* problem, int32_t sink_size, int32_t seq, int32_t m0, int32_t m1,
+                                int32_t* out, int32_t max_blocks);
+int b200fa_sink_query_blocks_host(const b200fa_problem* problem, int32_t sink_size, int32_t seq, int32_t c0, int32_t c1,
+                                  int32_t* out, int32_t max_blocks);
+
 /* ---- Paged key-value cache (no counterpart in the reference).
  * A cache tensor is (num_pages, page_size, heads_kv, head_dim) BF16; key j of sequence b is row j % page_size of page
  * block_table[b][j / page_size]. A table entry outside [0, num_pages) holds no page: its positions are not visible, and

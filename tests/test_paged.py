@@ -56,13 +56,17 @@ def decode_arguments(**changes):
     (dict(cache_seqlens=ints(2)), "cache_seqlens must be an int32 tensor"),
     (dict(window_left=-2), "window bounds"),
     (dict(sink_size=-1), "sink_size"),
-    (dict(sink_size=1.5), "sink_size"),
     (dict(cache_seqlens=ints(3).to("meta")), "is on meta"),
 ])
 def test_decode_refusals(changes, message):
     paged.check_paged(**decode_arguments())
     with pytest.raises(ValueError, match=message):
         paged.check_paged(**decode_arguments(**changes))
+
+
+def test_decode_refuses_a_sink_size_that_is_no_integer():
+    with pytest.raises(TypeError, match="sink_size"):
+        paged.check_paged(**decode_arguments(sink_size=1.5))
 
 
 def test_decode_refuses_gradients():

@@ -128,8 +128,8 @@ int* device_status_word() {
 static std::atomic<long long*> g_trace{nullptr};
 long long* trace_buffer() { return g_trace.load(std::memory_order_relaxed); }
 
-int launch_fwd(const b200fa_fwd_args& args, cudaStream_t stream);
-int launch_bwd(const b200fa_bwd_args& args, cudaStream_t stream);
+int launch_fwd(const b200fa_fwd_args& args, int sink, cudaStream_t stream);
+int launch_bwd(const b200fa_bwd_args& args, int sink, cudaStream_t stream);
 size_t bwd_workspace_bytes(const b200fa_problem& problem);
 void arm_bwd_timing(void* const* events);
 
@@ -143,6 +143,21 @@ static int validate_problem(const b200fa_problem& p) {
   if (p.visibility_bits) {
     B200FA_REQUIRE(p.cu_seqlens_q && p.visibility_bits_t && p.cu_visible_k && p.cu_visible_q,
                    "inter-sequence attention needs cu_seqlens and the prepared metadata");
+  }
+  return B200FA_OK;
+}
+
+// Sinks matter in front of a window only: without a left bound every key is visible anyway.
+static int sinks_of(const b200fa_problem& p, int sink_size) { return p.window_left < 0 ? 0 : sink_size; }
+
+static int validate_sinks(const b200fa_problem& p, int sink_size) {
+  B200FA_REQUIRE(sink_size >= 0, "sink_size must not be negative");
+  B200FA_REQUIRE(sink_size == 0 || !p.visibility_bits, "inter-sequence attention has no sinks");
+  // masked scores are -inf before they are scaled
+  B200FA_REQUIRE(sinks_of(p, sink_size) == 0 || p.softmax_scale > 0.f, "attention with sinks needs a positive softmax_scale");
+  if (sinks_of(p, sink_size) > 0 && p.head_dim > 128) {
+    set_error("attention with sinks supports head_dim 64, 72, 96 and 128, got %d", p.head_dim);
+    return B200FA_ERR_UNSUPPORTED;
   }
   return B200FA_OK;
 }
@@ -180,20 +195,25 @@ int b200fa_device_status(void) {
   return status;
 }
 
-size_t b200fa_fwd_workspace_bytes(const b200fa_problem* p) {
-  if (!p->cu_seqlens_q) return fwd_split_workspace_bytes(*p);  // partial results of the split-KV path, usually 0
+size_t b200fa_fwd_workspace_bytes(const b200fa_problem* p) { return b200fa_sink_fwd_workspace_bytes(p, 0); }
+
+size_t b200fa_sink_fwd_workspace_bytes(const b200fa_problem* p, int32_t sink_size) {
+  if (!p->cu_seqlens_q) return fwd_split_workspace_bytes(*p, sinks_of(*p, sink_size));  // partial results of the split-KV path, usually 0
   // work-list entries cover 256 query rows, 128 at head_dim 256 and 512, 256 >> shift tokens where query heads are packed
   const int tile_rows = p->head_dim >= 256 ? kBlockM : kFwdTileM >> fwd_pack_shift(*p);
   return static_cast<size_t>(work_list_entries(p->seqlen_q, p->batch, tile_rows)) * 8;
 }
 
-int b200fa_fwd(const b200fa_fwd_args* args, void* stream) {
+int b200fa_fwd(const b200fa_fwd_args* args, void* stream) { return b200fa_sink_fwd(args, 0, stream); }
+
+int b200fa_sink_fwd(const b200fa_fwd_args* args, int32_t sink_size, void* stream) {
   if (!args) {
     set_error("null arguments");
     return B200FA_ERR_INVALID;
   }
   const b200fa_problem& p = args->problem;
   int status = validate_problem(p);
+  if (status == B200FA_OK) status = validate_sinks(p, sink_size);
   if (status != B200FA_OK) return status;
   B200FA_REQUIRE(strides_ok(args->q_stride) && strides_ok(args->k_stride) && strides_ok(args->v_stride) &&
                      strides_ok(args->out_stride),
@@ -202,7 +222,7 @@ int b200fa_fwd(const b200fa_fwd_args* args, void* stream) {
   if (p.batch == 0 || p.seqlen_q == 0) return B200FA_OK;
   B200FA_REQUIRE(args->q && args->out && args->softmax_lse, "null tensor pointer");
   B200FA_REQUIRE(p.seqlen_k == 0 || (args->k && args->v), "null tensor pointer");
-  return launch_fwd(*args, static_cast<cudaStream_t>(stream));
+  return launch_fwd(*args, sinks_of(p, sink_size), static_cast<cudaStream_t>(stream));
 }
 
 int b200fa_set_trace(void* counters) {
@@ -222,13 +242,18 @@ int b200fa_bwd_timing_events(void* const* events) {
 
 size_t b200fa_bwd_workspace_bytes(const b200fa_problem* p) { return bwd_workspace_bytes(*p); }
 
-int b200fa_bwd(const b200fa_bwd_args* args, void* stream) {
+size_t b200fa_sink_bwd_workspace_bytes(const b200fa_problem* p, int32_t) { return bwd_workspace_bytes(*p); }
+
+int b200fa_bwd(const b200fa_bwd_args* args, void* stream) { return b200fa_sink_bwd(args, 0, stream); }
+
+int b200fa_sink_bwd(const b200fa_bwd_args* args, int32_t sink_size, void* stream) {
   if (!args) {
     set_error("null arguments");
     return B200FA_ERR_INVALID;
   }
   const b200fa_problem& p = args->problem;
   int status = validate_problem(p);
+  if (status == B200FA_OK) status = validate_sinks(p, sink_size);
   if (status != B200FA_OK) return status;
   B200FA_REQUIRE(strides_ok(args->q_stride) && strides_ok(args->k_stride) && strides_ok(args->v_stride) &&
                      strides_ok(args->out_stride) && strides_ok(args->dout_stride) && strides_ok(args->dq_stride) &&
@@ -246,7 +271,7 @@ int b200fa_bwd(const b200fa_bwd_args* args, void* stream) {
   for (const void* pointer : aligned16)
     B200FA_REQUIRE(reinterpret_cast<uintptr_t>(pointer) % 16 == 0, "tensor pointers must be 16-byte aligned");
   B200FA_REQUIRE(reinterpret_cast<uintptr_t>(args->softmax_lse) % 4 == 0, "softmax_lse must be 4-byte aligned");
-  return launch_bwd(*args, static_cast<cudaStream_t>(stream));
+  return launch_bwd(*args, sinks_of(p, sink_size), static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

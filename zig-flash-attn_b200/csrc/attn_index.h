@@ -84,6 +84,12 @@ B200FA_HD void band_query_block_range(const Band& band, int lq, int c0, int c1, 
   *last = ceil_div(hi, kBlockM);
 }
 
+// The same with the first `sink` columns visible to every row that the right bound lets see them.
+B200FA_HD void sink_query_block_range(Band band, int lq, int c0, int c1, int sink, int* first, int* last) {
+  if (c0 < sink) band.left = -1;
+  band_query_block_range(band, lq, c0, c1, first, last);
+}
+
 // Problem description common to forward and backward kernels (plain data; passed by value to kernels).
 struct Problem {
   int batch;        // batch entries (fixed length) or sequences (varlen / inter-sequence)
@@ -98,6 +104,7 @@ struct Problem {
   const int32_t* bits_t;        // transpose
   const int32_t* window_sizes;  // (2, n) or null
   int words;
+  int sink;                     // the first `sink` keys stay visible in front of the window (instances with kSink)
 };
 
 struct SeqInfo {
@@ -149,8 +156,11 @@ struct OtherBlock {
 // kBits = false compiles the visibility-bit scan out (problems without bits: fixed length and plain packed batches);
 // the forward kernel at head_dim <= 128 has an instance of its own for them, because the scan code inlined into its
 // three roles costs short sequences a few percent even when it never runs.
-template <bool kBits>
+// kSink = true adds the sinks of window attention: key blocks that hold one of the first `sink` keys come before those of
+// the window. `blk` then counts the visited blocks, and those behind the first `sink_blocks` lie `gap` blocks further on.
+template <bool kBits, bool kSink = false>
 struct KeyCursorT {
+  static_assert(!(kBits && kSink), "inter-sequence batches have no sinks");
   const Problem* p;
   int seq, m0, m1;
   Band band;       // band of the sequence itself
@@ -158,6 +168,7 @@ struct KeyCursorT {
   // current run
   int run_row0, run_len, run_banded;
   int blk, blk_end;
+  int sink_blocks, gap;  // kSink only
   // scan position over key sequences (inter-sequence only); -1 = finished
   int scan;
 
@@ -181,6 +192,13 @@ struct KeyCursorT {
       run_len = s.lk;
       run_banded = 1;
       band_key_block_range(band, m0, m1, &blk, &blk_end);
+      if (kSink) {
+        const int sinks = blk_end > blk ? imin(p->sink, imin(s.lk, band.hi(m1 - 1))) : 0;
+        sink_blocks = imin(ceil_div(sinks, kBlockN), blk);
+        gap = blk - sink_blocks;
+        blk_end -= gap;
+        blk = 0;
+      }
     } else {
       self_banded = !band.unbounded();
       scan = 0;
@@ -245,8 +263,9 @@ struct KeyCursorT {
     if (blk >= blk_end) {
       if (!kBits || scan < 0 || !next_run()) return false;
     }
-    out->row = run_row0 + blk * kBlockN;
-    out->col0 = blk * kBlockN;
+    const int at = kSink && blk >= sink_blocks ? blk + gap : blk;
+    out->row = run_row0 + at * kBlockN;
+    out->col0 = at * kBlockN;
     out->limit = run_len;
     out->banded = run_banded;
     ++blk;
@@ -260,8 +279,11 @@ using KeyCursor = KeyCursorT<true>;
 // [c0, c1) of key sequence `seq`, in increasing query order. Uses the transposed visibility bits.
 // kBits = false compiles the scan of the transposed visibility bits out. The backward kernels use the full cursor:
 // an instance without the scan measured 1-3 % slower there, unlike in the forward kernel.
-template <bool kBits>
+// kSink = true: a key block that holds one of the first `sink` keys is seen by every query row that the right bound lets
+// see it, so its range of query blocks ends with the sequence, not with the window.
+template <bool kBits, bool kSink = false>
 struct QueryCursorT {
+  static_assert(!(kBits && kSink), "inter-sequence batches have no sinks");
   const Problem* p;
   int seq, c0, c1;
   Band band;
@@ -291,7 +313,11 @@ struct QueryCursorT {
       run_row0 = s.q0;
       run_len = s.lq;
       run_banded = 1;
-      band_query_block_range(band, s.lq, c0, c1, &blk, &blk_end);
+      if (kSink) {
+        sink_query_block_range(band, s.lq, c0, c1, p->sink, &blk, &blk_end);
+      } else {
+        band_query_block_range(band, s.lq, c0, c1, &blk, &blk_end);
+      }
     } else {
       self_banded = !band.unbounded();
       scan = 0;

@@ -68,12 +68,22 @@ struct BwdConfig {
   static constexpr int kTmemS = 0, kTmemDp = 128, kTmemDv = 256, kTmemDk = 256 + D;
 };
 
-template <int D, bool kPivot>
+// Zeroes row r of a 128-row tile of D columns (panels of 64 columns, 128 bytes a row; the swizzle stays within a row).
+template <int D>
+__device__ __forceinline__ void zero_row(uint32_t tile, int r) {
+#pragma unroll 1
+  for (int i = 0; i < D / 8; ++i) st_shared_zero16(tile + (i >> 3) * (kBlockM * 128) + r * 128 + (i & 7) * 16);
+}
+
+// kSink: window attention whose first keys stay visible (b200fa_sink_bwd), an instance of its own so that the others keep
+// their code.
+template <int D, bool kPivot, bool kSink>
 __global__ void __launch_bounds__(BwdConfig<D>::kThreads, 1)
 bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
            const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_do,
            const __grid_constant__ CUtensorMap map_dq, const __grid_constant__ BwdParams p) {
   using Cfg = BwdConfig<D>;
+  using Cursor = QueryCursorT<!kSink, kSink>;
   const Problem& pr = p.prob;
   // ---- work item (uniform over the CTA; exits before any barrier or TMEM allocation)
   int seq, n_block, kv_head;
@@ -152,7 +162,7 @@ bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CU
   // Query blocks per head (the same for every head of the group).
   int blocks_per_head = 0;
   {
-    QueryCursor cur;
+    Cursor cur;
     cur.init(&pr, seq, s, n0, c1);
     OtherBlock qb;
     while (cur.next(&qb)) ++blocks_per_head;
@@ -182,7 +192,7 @@ bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CU
       const int head = kv_head * group + g;
       const float* lse_head = p.lse_log2 + (int64_t)head * p.rows;
       const float* dpsum_head = p.dpsum + (int64_t)head * p.rows;
-      QueryCursor cur;
+      Cursor cur;
       cur.init(&pr, seq, s, n0, c1);
       OtherBlock qb;
       while (cur.next(&qb)) {
@@ -332,7 +342,7 @@ bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CU
     int it = 0;
     bool ok = true;
     for (int g = 0; ok && g < group; ++g) {
-      QueryCursor cur;
+      Cursor cur;
       cur.init(&pr, seq, s, n0, c1);
       OtherBlock qb;
       while (cur.next(&qb)) {
@@ -340,13 +350,28 @@ bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CU
         int qlo = 0, qhi = qb.limit - qb.col0;
         if (qb.banded) {
           if (right >= 0) qlo = imax(0, c - off - right - qb.col0);
-          if (left >= 0) qhi = imin(qhi, c - off + left + 1 - qb.col0);
+          if (left >= 0 && !(kSink && c < pr.sink)) qhi = imin(qhi, c - off + left + 1 - qb.col0);
         }
         if (!key_valid) qhi = 0;
         const bool masked = __any_sync(0xffffffffu, qlo > cb || qhi < cb + C);
         // ---- P^T (kept in FP32 registers for dS, stored to TMEM as BF16 for the dV MMA)
         if (!mbar_wait_traced(bar_s_full, it & 1, wctx, kWaitBwdCompute, 7, true)) { ok = false; break; }
         tc_fence_after();
+        if constexpr (kSink) {
+          // Rows of the tiles behind the end of a packed sequence belong to the next one or to nobody, so anything may
+          // stand there. Their P and dS are 0, but 0 x NaN is not: the K rows (dQ reads them), the Q rows (dK) and the dO
+          // rows (dV) become zeros before the barriers that those products wait for. dO is touched once dP^T has read it.
+          if (pr.cu_q && it == 0 && wg == 0 && !key_valid) zero_row<D>(smem_k, r);
+          if (pr.cu_q && qb.limit - qb.col0 < kBlockM) {
+            if (!mbar_wait(bar_dp_full, it & 1, wctx, kWaitBwdCompute)) { ok = false; break; }
+            if (wg == 0 && r >= qb.limit - qb.col0) {
+              zero_row<D>(smem_q + st * Cfg::kTileBytes, r);
+              zero_row<D>(smem_do, r);
+            }
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+        }
         const long long t_p = trace_clock(wctx);
         trace_event(wctx, traced_cta && threadIdx.x == 0 && it < 10, 1, trace_n, 500 + it);  // S ready
         trace_event(wctx, traced_cta && threadIdx.x == 32 * Cfg::kComputeWarps - 32 && it < 10, 4, trace_n, 1500 + it);  // the same from the last compute warp
@@ -524,7 +549,7 @@ bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CU
     bool ok = true;
     for (int g = 0; ok && g < group; ++g) {
       const int head = kv_head * group + g;
-      QueryCursor cur;
+      Cursor cur;
       cur.init(&pr, seq, s, n0, c1);
       OtherBlock qb;
       while (cur.next(&qb)) {
@@ -895,24 +920,26 @@ static int launch_main(const b200fa_bwd_args& a, const BwdParams& p, dim3 grid, 
     if (status != B200FA_OK) return status;
   }
 
-  if (p.pivot_key) {
-    static bool attribute_set[64] = {false};
-    status = set_dynamic_smem_once(reinterpret_cast<const void*>(&bwd_kernel<D, true>), Cfg::kSmemBytes, attribute_set);
-    if (status != B200FA_OK) return status;
-    bwd_kernel<D, true><<<grid, Cfg::kThreads, Cfg::kSmemBytes, stream>>>(map_q, map_k, map_v, map_do, map_dq, p);
+  auto launch = [&](auto kernel, bool (&attribute_set)[64]) -> int {
+    const int set = set_dynamic_smem_once(reinterpret_cast<const void*>(kernel), Cfg::kSmemBytes, attribute_set);
+    if (set != B200FA_OK) return set;
+    kernel<<<grid, Cfg::kThreads, Cfg::kSmemBytes, stream>>>(map_q, map_k, map_v, map_do, map_dq, p);
+    return B200FA_OK;
+  };
+  static bool set_plain[64] = {false}, set_pivot[64] = {false}, set_sink[64] = {false}, set_sink_pivot[64] = {false};
+  if (p.prob.sink > 0) {
+    status = p.pivot_key ? launch(&bwd_kernel<D, true, true>, set_sink_pivot) : launch(&bwd_kernel<D, false, true>, set_sink);
   } else {
-    static bool attribute_set[64] = {false};
-    status = set_dynamic_smem_once(reinterpret_cast<const void*>(&bwd_kernel<D, false>), Cfg::kSmemBytes, attribute_set);
-    if (status != B200FA_OK) return status;
-    bwd_kernel<D, false><<<grid, Cfg::kThreads, Cfg::kSmemBytes, stream>>>(map_q, map_k, map_v, map_do, map_dq, p);
+    status = p.pivot_key ? launch(&bwd_kernel<D, true, false>, set_pivot) : launch(&bwd_kernel<D, false, false>, set_plain);
   }
+  if (status != B200FA_OK) return status;
   B200FA_CUDA_CHECK(cudaGetLastError());
 
   return B200FA_OK;
 }
 
 template <int D>
-static int launch_bwd_d(const b200fa_bwd_args& a, cudaStream_t stream) {
+static int launch_bwd_d(const b200fa_bwd_args& a, int sink, cudaStream_t stream) {
   const b200fa_problem& bp = a.problem;
   const bool packed = bp.cu_seqlens_q != nullptr;
   const BwdWorkspace w = plan_workspace(bp);
@@ -947,6 +974,7 @@ static int launch_bwd_d(const b200fa_bwd_args& a, cudaStream_t stream) {
 
   BwdParams p;
   p.prob = to_problem(bp);
+  p.prob.sink = sink;
   p.scale = bp.softmax_scale;
   p.scale_log2 = bp.softmax_scale * kLog2e;
   p.lse_log2 = lse_log2;
@@ -1000,7 +1028,7 @@ static int launch_bwd_d(const b200fa_bwd_args& a, cudaStream_t stream) {
     for (int nb = 0; nb < p.n_blocks; ++nb) {
       int first = 0, last = 0;
       const int c0 = nb * kBlockN, c1 = c0 + kBlockN < bp.seqlen_k ? c0 + kBlockN : bp.seqlen_k;
-      band_query_block_range(band, bp.seqlen_q, c0, c1, &first, &last);
+      sink_query_block_range(band, bp.seqlen_q, c0, c1, sink, &first, &last);
       const int64_t weight = last > first ? last - first : 0;
       total_weight += weight;
       heaviest = weight > heaviest ? weight : heaviest;
@@ -1058,16 +1086,16 @@ static int launch_bwd_d(const b200fa_bwd_args& a, cudaStream_t stream) {
   return B200FA_OK;
 }
 
-int launch_bwd(const b200fa_bwd_args& a, cudaStream_t stream) {
+int launch_bwd(const b200fa_bwd_args& a, int sink, cudaStream_t stream) {
   switch (a.problem.head_dim) {
     case 64:
-      return launch_bwd_d<64>(a, stream);
+      return launch_bwd_d<64>(a, sink, stream);
     case 72:   // compiled for 128 columns; TMA zero-fills the missing ones and the epilogues skip them
     case 96:
     case 128:
-      return launch_bwd_d<128>(a, stream);
+      return launch_bwd_d<128>(a, sink, stream);
     case 256:
-      return launch_bwd_d<256>(a, stream);
+      return launch_bwd_d<256>(a, sink, stream);
     default:
       set_error("head_dim %d is not supported by the backward kernels (supported: 64, 72, 96, 128, 256)", a.problem.head_dim);
       return B200FA_ERR_UNSUPPORTED;

@@ -49,7 +49,10 @@ struct FwdConfig {
   static constexpr int kPStride = kOwnP ? 64 : 128;          // columns between the P of the two stages
 };
 
-template <int D, bool kSplit, bool kBits>
+// kSink: window attention whose first keys stay visible (b200fa_sink_fwd). Its key blocks are those of the sinks and of
+// the window, and a block's mask has two intervals. An instance of its own, because the second compare per score and the
+// longer cursor would cost every masked block of the others.
+template <int D, bool kSplit, bool kBits, bool kSink>
 __global__ void __launch_bounds__(FwdConfig<D>::kThreads, 1)
 fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
            const __grid_constant__ CUtensorMap map_v, const __grid_constant__ FwdParams p) {
@@ -162,7 +165,7 @@ fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CU
       for (int tile; ok && (tile = tiles.push(drawn, p.tile_counter, p.num_tiles, wctx)) >= 0;) {
         FwdTile t = decode_tile(p, tile / splits);
         if (!t.valid) continue;
-        KeyCursorT<kBits> cur;
+        KeyCursorT<kBits, kSink> cur;
         cur.init(&pr, t.seq, t.s, t.m0, imin(t.m0 + (kFwdTileM >> p.pack_shift), t.s.lq));
         if (kSplit) cur.restrict_to_share(tile % splits, splits);
         OtherBlock kb;
@@ -232,7 +235,7 @@ fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CU
       for (int tile; ok && (tile = tiles.pop_thread(popped, wctx)) >= 0;) {
         FwdTile t = decode_tile(p, tile / splits);
         if (!t.valid) continue;
-        KeyCursorT<kBits> cur;
+        KeyCursorT<kBits, kSink> cur;
         cur.init(&pr, t.seq, t.s, t.m0, imin(t.m0 + (kFwdTileM >> p.pack_shift), t.s.lq));
         if (kSplit) cur.restrict_to_share(tile % splits, splits);
         OtherBlock kb;
@@ -348,7 +351,7 @@ fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CU
       const int tile_row = stage * kBlockM + row_in_stage;
       const int row = t.m0 + (tile_row >> p.pack_shift);
       const int head = t.head + (tile_row & ((1 << p.pack_shift) - 1));
-      KeyCursorT<kBits> cur;
+      KeyCursorT<kBits, kSink> cur;
       cur.init(&pr, t.seq, t.s, t.m0, imin(t.m0 + (kFwdTileM >> p.pack_shift), t.s.lq));
       const int split = kSplit ? tile % splits : 0;
       if (kSplit) cur.restrict_to_share(split, splits);
@@ -376,13 +379,31 @@ fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CU
           lo = 0;
           hi = kb.limit - kb.col0;
         }
+        const int sinks = kSink ? pr.sink - kb.col0 : 0;  // columns of this block that hold sinks
+        if (kSink && sinks >= lo) lo = 0;
         const bool masked = __any_sync(0xffffffffu, lo > 0 || hi < kBlockN);
+        if (kSink && stage == 0 && pr.cu_k && kb.limit - kb.col0 < kBlockN) {
+          // The last block of a packed sequence reaches into rows of the next one, or behind the last one, where anything
+          // may stand; their probabilities are 0, but 0 x NaN is not. Their V rows become zeros before the product reads
+          // them: the MMA thread issues the products of both stages behind the P barriers of this one. (The wait is valid
+          // without having followed the barrier: the scores being present proves the slot's previous use complete.)
+          const uint32_t v_index = ring + 2 * tile_blocks + 1;
+          if (!mbar_wait(bar_kv_full + 8 * (v_index % NS), (v_index / NS) & 1, wctx, kWaitKvFull)) { ok = false; break; }
+          if (row_in_stage >= kb.limit - kb.col0) {
+            const uint32_t v_row = smem_kv + (v_index % NS) * Cfg::kTileBytes + row_in_stage * 128;
+#pragma unroll 1
+            for (int i = 0; i < Cfg::kHalves * 8; ++i)
+              st_shared_zero16(v_row + (i >> 3) * Cfg::kPanelBytes + (i & 7) * 16);
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+        }
         auto apply_mask = [&](float2* values, int first_column) {
 #pragma unroll
           for (int i = 0; i < 32; ++i) {
             const int c = first_column + 2 * i;
-            values[i].x = (c >= lo && c < hi) ? values[i].x : -INFINITY;
-            values[i].y = (c + 1 >= lo && c + 1 < hi) ? values[i].y : -INFINITY;
+            values[i].x = column_visible<kSink>(c, lo, hi, sinks) ? values[i].x : -INFINITY;
+            values[i].y = column_visible<kSink>(c + 1, lo, hi, sinks) ? values[i].y : -INFINITY;
           }
         };
         auto max_of = [&](const float2* values) {
@@ -457,8 +478,8 @@ fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CU
           // carries no compare per score.
           counting = __any_sync(0xffffffffu, set_apart);
           if (__builtin_expect(counting, 0))
-            sum_counted = sum_without_keys_apart<kBlockN>(top, l, set_apart, block_max, t_s, masked, lo, hi, scale_log2,
-                                                          (m == -INFINITY) ? 0.f : m * scale_log2);
+            sum_counted = sum_without_keys_apart<kBlockN, kSink>(top, l, set_apart, block_max, t_s, masked, lo, hi,
+                                                                 scale_log2, (m == -INFINITY) ? 0.f : m * scale_log2, sinks);
         }
         const float mc = (m == -INFINITY) ? 0.f : m * scale_log2;
         const float2 scale2 = make_float2(scale_log2, scale_log2), shift2 = make_float2(-mc, -mc);
@@ -678,14 +699,14 @@ struct SplitPlan {
   int splits;
   size_t o_bytes, lse_bytes;
 };
-static SplitPlan plan_split(const b200fa_problem& bp) {
+static SplitPlan plan_split(const b200fa_problem& bp, int sink) {
   SplitPlan plan{1, 0, 0};
   if (bp.cu_seqlens_q || bp.visibility_bits || bp.head_dim > 128 || bp.batch <= 0 || bp.seqlen_q <= 0) return plan;
   const int tile_tokens = kFwdTileM >> pack_shift_of(bp);
   const int64_t tiles = (int64_t)bp.batch * (bp.heads_q >> pack_shift_of(bp)) * ceil_div(bp.seqlen_q, tile_tokens);
   int64_t keys = bp.seqlen_k;
   if (bp.window_left >= 0) {
-    const int64_t reach = (int64_t)bp.window_left + imin(bp.seqlen_q, tile_tokens) + imax(bp.window_right, 0);
+    const int64_t reach = (int64_t)bp.window_left + imin(bp.seqlen_q, tile_tokens) + imax(bp.window_right, 0) + sink;
     keys = keys < reach ? keys : reach;
   }
   const int64_t blocks = (keys + kBlockN - 1) / kBlockN;
@@ -701,8 +722,8 @@ static SplitPlan plan_split(const b200fa_problem& bp) {
   plan.lse_bytes = ((size_t)splits * rows * bp.heads_q * 4 + 255) & ~size_t(255);
   return plan;
 }
-size_t fwd_split_workspace_bytes(const b200fa_problem& bp) {
-  const SplitPlan plan = plan_split(bp);
+size_t fwd_split_workspace_bytes(const b200fa_problem& bp, int sink) {
+  const SplitPlan plan = plan_split(bp, sink);
   return plan.o_bytes + plan.lse_bytes;
 }
 
@@ -757,7 +778,7 @@ __global__ void __launch_bounds__(256) split_combine_kernel(const float* __restr
 
 int prepare_forward(const b200fa_fwd_args& a, cudaStream_t stream, int head_dim, int tile_rows, int kv_box_rows,
                     FwdParams* params, CUtensorMap* map_q, CUtensorMap* map_k, CUtensorMap* map_v, bool* nothing_to_do,
-                    int v_box_rows, int pack_shift) {
+                    int v_box_rows, int pack_shift, int sink) {
   const b200fa_problem& bp = a.problem;
   const int D = bp.head_dim;  // columns of the tensors; `head_dim` is the width the kernel is compiled for
   (void)head_dim;
@@ -765,6 +786,7 @@ int prepare_forward(const b200fa_fwd_args& a, cudaStream_t stream, int head_dim,
   FwdParams& p = *params;
   *nothing_to_do = true;
   p.prob = to_problem(bp);
+  p.prob.sink = sink;
   p.scale_log2 = bp.softmax_scale * 1.4426950408889634f;
   p.o = static_cast<__nv_bfloat16*>(a.out);
   p.o_batch_stride = packed ? 0 : a.out_stride[0];
@@ -850,13 +872,13 @@ int prepare_forward(const b200fa_fwd_args& a, cudaStream_t stream, int head_dim,
 }
 
 template <int D>
-static int launch_fwd_d(const b200fa_fwd_args& a, cudaStream_t stream) {
+static int launch_fwd_d(const b200fa_fwd_args& a, int sink, cudaStream_t stream) {
   using Cfg = FwdConfig<D>;
   FwdParams p;
   CUtensorMap map_q, map_k, map_v;
   bool nothing_to_do = false;
   int status = prepare_forward(a, stream, D, kFwdTileM, kBlockN, &p, &map_q, &map_k, &map_v, &nothing_to_do, 0,
-                               pack_shift_of(a.problem));
+                               pack_shift_of(a.problem), sink);
   if (status != B200FA_OK || nothing_to_do) return status;
   int sms = 0;
   status = device_sm_count(&sms);
@@ -864,7 +886,7 @@ static int launch_fwd_d(const b200fa_fwd_args& a, cudaStream_t stream) {
   // Split-KV when the plan asks for it and the caller's workspace has room for the partial results (an entry point
   // that brings its own small scratch runs the same problem unsplit).
   const b200fa_problem& bp = a.problem;
-  const SplitPlan plan = plan_split(bp);
+  const SplitPlan plan = plan_split(bp, sink);
   const bool split = plan.splits > 1 && a.workspace && a.workspace_bytes >= plan.o_bytes + plan.lse_bytes &&
                      reinterpret_cast<uintptr_t>(a.workspace) % 16 == 0;
   if (split) {
@@ -875,7 +897,8 @@ static int launch_fwd_d(const b200fa_fwd_args& a, cudaStream_t stream) {
     p.num_tiles *= plan.splits;
   }
   const int grid = p.num_tiles < sms ? p.num_tiles : sms;
-  // Three instances: split-KV, problems with visibility bits (inter-sequence batches), and the plain one.
+  // Instances: split-KV, problems with visibility bits (inter-sequence batches), the plain one, and the first and the
+  // last of these with sinks.
   auto launch = [&](auto kernel, bool (&attribute_set)[64]) -> int {
     const int set = set_dynamic_smem_once(reinterpret_cast<const void*>(kernel), Cfg::kSmemBytes, attribute_set);
     if (set != B200FA_OK) return set;
@@ -883,12 +906,16 @@ static int launch_fwd_d(const b200fa_fwd_args& a, cudaStream_t stream) {
     return B200FA_OK;
   };
   static bool set_split[64] = {false}, set_bits[64] = {false}, set_plain[64] = {false};
-  if (split) {
-    status = launch(&fwd_kernel<D, true, false>, set_split);
+  static bool set_sink_split[64] = {false}, set_sink[64] = {false};
+  if (sink > 0) {
+    status = split ? launch(&fwd_kernel<D, true, false, true>, set_sink_split)
+                   : launch(&fwd_kernel<D, false, false, true>, set_sink);
+  } else if (split) {
+    status = launch(&fwd_kernel<D, true, false, false>, set_split);
   } else if (bp.visibility_bits) {
-    status = launch(&fwd_kernel<D, false, true>, set_bits);
+    status = launch(&fwd_kernel<D, false, true, false>, set_bits);
   } else {
-    status = launch(&fwd_kernel<D, false, false>, set_plain);
+    status = launch(&fwd_kernel<D, false, false, false>, set_plain);
   }
   if (status != B200FA_OK) return status;
   B200FA_CUDA_CHECK(cudaGetLastError());
@@ -903,14 +930,14 @@ static int launch_fwd_d(const b200fa_fwd_args& a, cudaStream_t stream) {
   return B200FA_OK;
 }
 
-int launch_fwd(const b200fa_fwd_args& a, cudaStream_t stream) {
+int launch_fwd(const b200fa_fwd_args& a, int sink, cudaStream_t stream) {
   switch (a.problem.head_dim) {
     case 64:
-      return launch_fwd_d<64>(a, stream);
+      return launch_fwd_d<64>(a, sink, stream);
     case 72:   // compiled for 128 columns; TMA zero-fills the missing ones and the epilogue skips them
     case 96:
     case 128:
-      return launch_fwd_d<128>(a, stream);
+      return launch_fwd_d<128>(a, sink, stream);
     case 256: {
       // B200FA_FWD_D256_PAIR=1 in the environment selects the two-CTA variant (same results bit for bit, measured
       // slower: kept for tuning work on `cta_group::2` tiles).

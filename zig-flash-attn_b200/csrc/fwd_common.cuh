@@ -68,6 +68,12 @@ __device__ __forceinline__ float log2p1_series(float x) {
   return 1.4426950408889634f * (x * series);
 }
 
+// Column c of a key block under the limits of its row: [lo, hi), and with kSink the columns below min(sinks, hi) too.
+template <bool kSink>
+__device__ __forceinline__ bool column_visible(int c, int lo, int hi, int sinks) {
+  return (c >= lo || (kSink && c < sinks)) && c < hi;
+}
+
 // Per-row state of the keys that the online softmax sets aside (see row_totals below): `ones` keys, all scoring exactly
 // `apart`, are kept out of the running sum. (Two registers: the softmax warps have none to spare, and a third one for
 // the running maximum of the row cost the masked blocks of causal problems 4 %.)
@@ -94,10 +100,10 @@ __device__ __forceinline__ bool sets_keys_apart(const TopApart& st, float part_a
 // `set_apart` is true for this thread, which it counts in st.ones instead. Keys set aside earlier at a lower score are
 // folded back into `l` first. A rolled loop over four columns at a time keeps the path small; `mc` is the reference
 // maximum times scale_log2 that the block's exponentials use. Returns the sum that replaces the block sum.
-template <int kColumns>
+template <int kColumns, bool kSink = false>
 __device__ __forceinline__ float sum_without_keys_apart(TopApart& st, float& l, bool set_apart, float block_max,
                                                         uint32_t t_s, bool masked, int lo, int hi, float scale_log2,
-                                                        float mc) {
+                                                        float mc, int sinks = 0) {
   float apart_here = __int_as_float(0x7fc00000);  // NaN: no score equals it
   if (set_apart) {
     if (block_max > st.apart) {  // the keys set aside earlier are ordinary terms from now on
@@ -116,8 +122,8 @@ __device__ __forceinline__ float sum_without_keys_apart(TopApart& st, float& l, 
     tc_wait_ld();
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const float sx = (!masked || (c + 2 * i >= lo && c + 2 * i < hi)) ? again[i].x : -INFINITY;
-      const float sy = (!masked || (c + 2 * i + 1 >= lo && c + 2 * i + 1 < hi)) ? again[i].y : -INFINITY;
+      const float sx = (!masked || column_visible<kSink>(c + 2 * i, lo, hi, sinks)) ? again[i].x : -INFINITY;
+      const float sy = (!masked || column_visible<kSink>(c + 2 * i + 1, lo, hi, sinks)) ? again[i].y : -INFINITY;
       const float2 x = __ffma2_rn(make_float2(sx, sy), scale2, shift2);
       const float ex = ex2_approx(x.x), ey = ex2_approx(x.y);
       ones += (sx == apart_here ? 1.f : 0.f) + (sy == apart_here ? 1.f : 0.f);
@@ -257,7 +263,8 @@ __device__ __forceinline__ FwdTile decode_tile(const FwdParams& p, int tile, int
 int prepare_forward(const b200fa_fwd_args& a, cudaStream_t stream, int head_dim, int tile_rows, int kv_box_rows,
                     FwdParams* p, CUtensorMap* map_q, CUtensorMap* map_k, CUtensorMap* map_v, bool* nothing_to_do,
                     int v_box_rows = 0 /* rows per TMA box of V when they differ from those of K */,
-                    int pack_shift = 0 /* log2 of the query heads packed into the rows of a work item */);
+                    int pack_shift = 0 /* log2 of the query heads packed into the rows of a work item */,
+                    int sink = 0 /* first keys that stay visible in front of the window (instances with kSink) */);
 // A zeroed work-item counter for one launch on `stream`: the next slot of the device's ring of 4096 counters inside the
 // library, reset by a memset node ahead of the kernel. Launches share a slot only 4096 launches apart (or through a
 // captured graph, which keeps its slot); see the contract at its definition in fwd.cu.

@@ -353,6 +353,9 @@ __device__ __forceinline__ void named_barrier_sync(int id, int threads) {
 __device__ __forceinline__ void st_shared_f32(uint32_t addr, float value) {
   asm volatile("st.shared.f32 [%0], %1;" ::"r"(addr), "f"(value) : "memory");
 }
+__device__ __forceinline__ void st_shared_zero16(uint32_t addr) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(addr), "r"(0) : "memory");
+}
 __device__ __forceinline__ float ld_shared_f32(uint32_t addr) {
   float value;
   asm volatile("ld.shared.f32 %0, [%1];" : "=f"(value) : "r"(addr) : "memory");

@@ -168,7 +168,25 @@ Problem to_problem(const b200fa_problem& in) {
   p.bits_t = in.visibility_bits_t;
   p.window_sizes = in.window_sizes;
   p.words = (in.batch + 31) / 32;
+  p.sink = 0;
   return p;
+}
+
+// Writes the blocks that a cursor hands out, four numbers each; returns how many there are.
+template <typename Cursor>
+static int list_blocks(Cursor& cursor, int32_t* out, int32_t max_blocks) {
+  OtherBlock block;
+  int count = 0;
+  while (cursor.next(&block)) {
+    if (count < max_blocks) {
+      out[4 * count] = block.row;
+      out[4 * count + 1] = block.col0;
+      out[4 * count + 2] = block.limit;
+      out[4 * count + 3] = block.banded;
+    }
+    ++count;
+  }
+  return count;
 }
 
 }  // namespace b200fa
@@ -269,18 +287,7 @@ int b200fa_key_blocks_host(const b200fa_problem* problem, int32_t seq, int32_t m
   SeqInfo s = seq_info(p, seq);
   KeyCursor cursor;
   cursor.init(&p, seq, s, m0, imin(m1, s.lq));
-  OtherBlock block;
-  int count = 0;
-  while (cursor.next(&block)) {
-    if (count < max_blocks) {
-      out[4 * count] = block.row;
-      out[4 * count + 1] = block.col0;
-      out[4 * count + 2] = block.limit;
-      out[4 * count + 3] = block.banded;
-    }
-    ++count;
-  }
-  return count;
+  return list_blocks(cursor, out, max_blocks);
 }
 
 int b200fa_query_blocks_host(const b200fa_problem* problem, int32_t seq, int32_t c0, int32_t c1, int32_t* out,
@@ -289,18 +296,27 @@ int b200fa_query_blocks_host(const b200fa_problem* problem, int32_t seq, int32_t
   SeqInfo s = seq_info(p, seq);
   QueryCursor cursor;
   cursor.init(&p, seq, s, c0, imin(c1, s.lk));
-  OtherBlock block;
-  int count = 0;
-  while (cursor.next(&block)) {
-    if (count < max_blocks) {
-      out[4 * count] = block.row;
-      out[4 * count + 1] = block.col0;
-      out[4 * count + 2] = block.limit;
-      out[4 * count + 3] = block.banded;
-    }
-    ++count;
-  }
-  return count;
+  return list_blocks(cursor, out, max_blocks);
+}
+
+int b200fa_sink_key_blocks_host(const b200fa_problem* problem, int32_t sink_size, int32_t seq, int32_t m0, int32_t m1,
+                                int32_t* out, int32_t max_blocks) {
+  Problem p = to_problem(*problem);
+  p.sink = sink_size;
+  SeqInfo s = seq_info(p, seq);
+  KeyCursorT<false, true> cursor;
+  cursor.init(&p, seq, s, m0, imin(m1, s.lq));
+  return list_blocks(cursor, out, max_blocks);
+}
+
+int b200fa_sink_query_blocks_host(const b200fa_problem* problem, int32_t sink_size, int32_t seq, int32_t c0, int32_t c1,
+                                  int32_t* out, int32_t max_blocks) {
+  Problem p = to_problem(*problem);
+  p.sink = sink_size;
+  SeqInfo s = seq_info(p, seq);
+  QueryCursorT<false, true> cursor;
+  cursor.init(&p, seq, s, c0, imin(c1, s.lk));
+  return list_blocks(cursor, out, max_blocks);
 }
 
 }  // extern "C"

@@ -32,6 +32,12 @@ EXPORTS = (
     "b200fa_interseq_metadata_host",
     "b200fa_key_blocks_host",
     "b200fa_query_blocks_host",
+    "b200fa_sink_fwd_workspace_bytes",
+    "b200fa_sink_fwd",
+    "b200fa_sink_bwd_workspace_bytes",
+    "b200fa_sink_bwd",
+    "b200fa_sink_key_blocks_host",
+    "b200fa_sink_query_blocks_host",
     "b200fa_paged_decode_workspace_bytes",
     "b200fa_paged_decode",
     "b200fa_paged_keys_host",
@@ -216,6 +222,15 @@ def library() -> ctypes.CDLL:
     lib.b200fa_key_blocks_host.argtypes = [ctypes.POINTER(Problem)] + [ctypes.c_int32] * 3 + [ctypes.c_void_p, ctypes.c_int32]
     lib.b200fa_query_blocks_host.restype = ctypes.c_int
     lib.b200fa_query_blocks_host.argtypes = [ctypes.POINTER(Problem)] + [ctypes.c_int32] * 3 + [ctypes.c_void_p, ctypes.c_int32]
+    for name, args in (("fwd", FwdArgs), ("bwd", BwdArgs)):
+        function = getattr(lib, f"b200fa_sink_{name}_workspace_bytes")
+        function.restype, function.argtypes = ctypes.c_size_t, [ctypes.POINTER(Problem), ctypes.c_int32]
+        function = getattr(lib, f"b200fa_sink_{name}")
+        function.restype, function.argtypes = ctypes.c_int, [ctypes.POINTER(args), ctypes.c_int32, ctypes.c_void_p]
+    for name in ("key", "query"):
+        function = getattr(lib, f"b200fa_sink_{name}_blocks_host")
+        function.restype = ctypes.c_int
+        function.argtypes = [ctypes.POINTER(Problem)] + [ctypes.c_int32] * 4 + [ctypes.c_void_p, ctypes.c_int32]
     lib.b200fa_paged_decode_workspace_bytes.restype = ctypes.c_size_t
     lib.b200fa_paged_decode_workspace_bytes.argtypes = [ctypes.POINTER(PagedArgs)]
     lib.b200fa_paged_decode.restype = ctypes.c_int

@@ -144,13 +144,14 @@ def _contiguous_int(tensor):
     return tensor if tensor is None or tensor.is_contiguous() else tensor.contiguous()
 
 
-def launch_forward(q, k, v, out, softmax_lse, cu_seqlens_q, cu_seqlens_k, softmax_scale, left, right, interseq=None):
-    """out, softmax_lse <- attention(q, k, v). `interseq` = (bits, bits_t, cu_visible_k, cu_visible_q, window_sizes)."""
+def launch_forward(q, k, v, out, softmax_lse, cu_seqlens_q, cu_seqlens_k, softmax_scale, left, right, interseq=None, sink=0):
+    """out, softmax_lse <- attention(q, k, v). `interseq` = (bits, bits_t, cu_visible_k, cu_visible_q, window_sizes);
+    `sink` = keys that stay visible in front of the window."""
     packed = cu_seqlens_q is not None
     library = _lib.library()
     problem = _lib.make_problem(q, k, cu_seqlens_q, cu_seqlens_k, softmax_scale, left, right, *(interseq or ()))
     with torch.cuda.device(q.device):
-        workspace = _workspace(library.b200fa_fwd_workspace_bytes(ctypes.byref(problem)), q.device)
+        workspace = _workspace(library.b200fa_sink_fwd_workspace_bytes(ctypes.byref(problem), sink), q.device)
         args = _lib.FwdArgs(
             problem=problem,
             q=q.data_ptr(),
@@ -166,17 +167,18 @@ def launch_forward(q, k, v, out, softmax_lse, cu_seqlens_q, cu_seqlens_k, softma
             workspace=workspace.data_ptr(),
             workspace_bytes=workspace.numel(),
         )
-        _lib.check(library.b200fa_fwd(ctypes.byref(args), _stream(q.device)))
+        _lib.check(library.b200fa_sink_fwd(ctypes.byref(args), sink, _stream(q.device)))
 
 
 def launch_backward(
-    dout, q, k, v, out, softmax_lse, dq, dk, dv, cu_seqlens_q, cu_seqlens_k, softmax_scale, left, right, interseq=None
+    dout, q, k, v, out, softmax_lse, dq, dk, dv, cu_seqlens_q, cu_seqlens_k, softmax_scale, left, right, interseq=None,
+    sink=0,
 ):
     packed = cu_seqlens_q is not None
     library = _lib.library()
     problem = _lib.make_problem(q, k, cu_seqlens_q, cu_seqlens_k, softmax_scale, left, right, *(interseq or ()))
     with torch.cuda.device(q.device):
-        workspace = _workspace(library.b200fa_bwd_workspace_bytes(ctypes.byref(problem)), q.device)
+        workspace = _workspace(library.b200fa_sink_bwd_workspace_bytes(ctypes.byref(problem), sink), q.device)
         strides = {
             name + "_stride": _lib.strides3(tensor, packed)
             for name, tensor in dict(q=q, k=k, v=v, out=out, dout=dout, dq=dq, dk=dk, dv=dv).items()
@@ -197,10 +199,10 @@ def launch_backward(
             workspace_bytes=workspace.numel(),
             **strides,
         )
-        _lib.check(library.b200fa_bwd(ctypes.byref(args), _stream(q.device)))
+        _lib.check(library.b200fa_sink_bwd(ctypes.byref(args), sink, _stream(q.device)))
 
 
-def forward_impl(q, k, v, cu_seqlens_q, cu_seqlens_k, softmax_scale, left, right, interseq=None, direction=FORWARD):
+def forward_impl(q, k, v, cu_seqlens_q, cu_seqlens_k, softmax_scale, left, right, interseq=None, direction=FORWARD, sink=0):
     check_inputs(q, k, v, cu_seqlens_q, cu_seqlens_k, direction)
     require_window(left, right)
     q, k, v = (readable(tensor) for tensor in (q, k, v))
@@ -209,13 +211,14 @@ def forward_impl(q, k, v, cu_seqlens_q, cu_seqlens_k, softmax_scale, left, right
     softmax_lse = q.new_empty(lse_shape(q, packed), dtype=torch.float32)
     launch_forward(
         q, k, v, out, softmax_lse, _contiguous_int(cu_seqlens_q), _contiguous_int(cu_seqlens_k), softmax_scale, left,
-        right, interseq,
+        right, interseq, sink,
     )
     return out, softmax_lse
 
 
 def backward_into(
-    dout, q, k, v, out, softmax_lse, cu_seqlens_q, cu_seqlens_k, softmax_scale, left, right, dq, dk, dv, interseq=None
+    dout, q, k, v, out, softmax_lse, cu_seqlens_q, cu_seqlens_k, softmax_scale, left, right, dq, dk, dv, interseq=None,
+    sink=0,
 ):
     packed = cu_seqlens_q is not None
     check_inputs(q, k, v, cu_seqlens_q, cu_seqlens_k, BACKWARD)
@@ -227,7 +230,7 @@ def backward_into(
     buffers = tuple(writable(tensor) for tensor in targets)
     launch_backward(
         dout, q, k, v, out, softmax_lse, *buffers, _contiguous_int(cu_seqlens_q), _contiguous_int(cu_seqlens_k),
-        softmax_scale, left, right, interseq,
+        softmax_scale, left, right, interseq, sink,
     )
     for target, buffer in zip(targets, buffers):
         if buffer is not target:
@@ -333,6 +336,71 @@ def flash_attn_backward_packed(
 @flash_attn_backward_packed.register_fake
 def _(*unused):
     return None
+
+
+# ---- sliding window with sinks
+def check_sink_size(sink_size):
+    if not isinstance(sink_size, numbers.Integral):
+        raise TypeError(f"sink_size must be an integer, got {type(sink_size).__name__}")
+    if not 0 <= sink_size < 2**31:
+        raise ValueError(f"sink_size must be non-negative and below 2**31, got {sink_size}")
+
+
+def check_same_device(reference, **tensors):
+    for name, tensor in tensors.items():
+        if tensor is not None and tensor.device != reference.device:
+            raise ValueError(f"{name} is on {tensor.device}, but the first tensor of the call is on {reference.device}")
+
+
+@torch.library.custom_op("zigfa::sink_forward", mutates_args=(), device_types="cuda")
+def sink_forward(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    cu_seqlens_q: torch.Tensor | None,
+    cu_seqlens_k: torch.Tensor | None,
+    softmax_scale: float,
+    window_size_left: int,
+    window_size_right: int,
+    sink_size: int,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    check_same_device(q, k=k, v=v, cu_seqlens_q=cu_seqlens_q, cu_seqlens_k=cu_seqlens_k)
+    check_sink_size(sink_size)
+    return forward_impl(q, k, v, cu_seqlens_q, cu_seqlens_k, softmax_scale, window_size_left, window_size_right, sink=sink_size)
+
+
+@sink_forward.register_fake
+def _(q, k, v, cu_seqlens_q, *unused):
+    return q.new_empty(q.shape), q.new_empty(lse_shape(q, cu_seqlens_q is not None), dtype=torch.float32)
+
+
+@torch.library.custom_op("zigfa::sink_backward", mutates_args=(), device_types="cuda")
+def sink_backward(
+    dout: torch.Tensor,
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    out: torch.Tensor,
+    softmax_lse: torch.Tensor,
+    cu_seqlens_q: torch.Tensor | None,
+    cu_seqlens_k: torch.Tensor | None,
+    softmax_scale: float,
+    window_size_left: int,
+    window_size_right: int,
+    sink_size: int,
+) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    check_same_device(q, dout=dout)
+    dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
+    backward_into(
+        dout, q, k, v, out, softmax_lse, cu_seqlens_q, cu_seqlens_k, softmax_scale, window_size_left,
+        window_size_right, dq, dk, dv, sink=sink_size,
+    )
+    return dq, dk, dv
+
+
+@sink_backward.register_fake
+def _(dout, q, k, v, *unused):
+    return q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
 
 
 # ---- inter-sequence
@@ -634,6 +702,31 @@ class FlashAttnVarlenKVPackedFunc(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dout, *unused):
         return _kvpacked_backward(ctx, dout)
+
+
+class FlashAttnSinkFunc(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, cu_seqlens_q, cu_seqlens_k, sink_size, softmax_scale, causal, window_size, deterministic,
+                return_attn_probs):
+        reject_unsupported(deterministic=deterministic)
+        check_sink_size(sink_size)
+        left, right = window_size
+        require_window(left, right)
+        softmax_scale = default_softmax_scale(softmax_scale, q.shape[-1])
+        if not softmax_scale > 0:
+            raise ValueError(f"attention with sinks needs a positive softmax_scale, got {softmax_scale}")
+        options = (softmax_scale, left, 0 if causal else right, sink_size)
+        out, softmax_lse = sink_forward(q, k, v, cu_seqlens_q, cu_seqlens_k, *options)
+        ctx.save_for_backward(q, k, v, out, softmax_lse, cu_seqlens_q, cu_seqlens_k)
+        ctx.options = options
+        if not return_attn_probs:
+            return out
+        ctx.mark_non_differentiable(softmax_lse)
+        return out, softmax_lse
+
+    @staticmethod
+    def backward(ctx, dout, *unused):
+        return _pad(ctx, *sink_backward(dout, *ctx.saved_tensors, *ctx.options))
 
 
 def _inter_sequence_window(causal, window_size, window_sizes):

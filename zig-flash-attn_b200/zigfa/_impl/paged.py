@@ -24,12 +24,6 @@ def _define(schema, implementation, fake):
 
 
 # ------------------------------------------------------------------------------------------------ validation
-def check_same_device(reference, **tensors):
-    for name, tensor in tensors.items():
-        if tensor is not None and tensor.device != reference.device:
-            raise ValueError(f"{name} is on {tensor.device}, but the first tensor of the call is on {reference.device}")
-
-
 def check_ints(name, tensor, *shape):
     """An int32 tensor of this shape (None: any size); a table's columns are contiguous, vectors may be strided."""
     if tensor.dtype != torch.int32 or tensor.dim() != len(shape) or any(
@@ -74,13 +68,8 @@ def check_paged(q, k_cache, v_cache, block_table, cache_seqlens, window_left, si
     check_ints("block_table", block_table, q.shape[0], None)
     check_ints("cache_seqlens", cache_seqlens, q.shape[0])
     ops.require_window(window_left, -1)
-    check_sink_size(sink_size)
-    check_same_device(q, k_cache=k_cache, v_cache=v_cache, block_table=block_table, cache_seqlens=cache_seqlens)
-
-
-def check_sink_size(sink_size):
-    if not isinstance(sink_size, int) or sink_size < 0:
-        raise ValueError(f"sink_size must be a non-negative integer, got {sink_size!r}")
+    ops.check_sink_size(sink_size)
+    ops.check_same_device(q, k_cache=k_cache, v_cache=v_cache, block_table=block_table, cache_seqlens=cache_seqlens)
 
 
 def check_append(k, v, k_cache, v_cache, block_table, cache_seqlens, cu_seqlens):
@@ -104,7 +93,7 @@ def check_append(k, v, k_cache, v_cache, block_table, cache_seqlens, cu_seqlens)
         check_ints("cu_seqlens", cu_seqlens, batch + 1)
     elif k.shape[0] != batch:
         raise ValueError("k, block_table and cache_seqlens must have the same number of sequences")
-    check_same_device(k, v=v, k_cache=k_cache, v_cache=v_cache, block_table=block_table, cache_seqlens=cache_seqlens,
+    ops.check_same_device(k, v=v, k_cache=k_cache, v_cache=v_cache, block_table=block_table, cache_seqlens=cache_seqlens,
                       cu_seqlens=cu_seqlens)
 
 
@@ -114,7 +103,7 @@ def check_copy(k_cache, v_cache, source_pages, target_pages):
         raise ValueError(f"head_dim must be a multiple of 8 of at most 1024, got {k_cache.shape[-1]}")
     check_ints("source_pages", source_pages, None)
     check_ints("target_pages", target_pages, source_pages.shape[0])
-    check_same_device(k_cache, v_cache=v_cache, source_pages=source_pages, target_pages=target_pages)
+    ops.check_same_device(k_cache, v_cache=v_cache, source_pages=source_pages, target_pages=target_pages)
 
 
 def check_books(block_table, page_refs, **per_sequence):
@@ -122,7 +111,7 @@ def check_books(block_table, page_refs, **per_sequence):
     check_ints("page_refs", page_refs, None)
     for name, tensor in per_sequence.items():
         check_ints(name, tensor, block_table.shape[0])
-    check_same_device(block_table, page_refs=page_refs, **per_sequence)
+    ops.check_same_device(block_table, page_refs=page_refs, **per_sequence)
 
 
 # ------------------------------------------------------------------------------------------------ launches
@@ -241,7 +230,7 @@ def reserve_pages(block_table, cache_seqlens, new_tokens, page_refs, page_size):
 def fork_pages(block_table, cache_seqlens, page_refs, parents, page_size):
     check_books(block_table, page_refs, cache_seqlens=cache_seqlens)
     check_ints("parents", parents, None)
-    check_same_device(block_table, parents=parents)
+    ops.check_same_device(block_table, parents=parents)
     check_page_size(page_size)
     rows = parents.shape[0]
     table, refs, source, target, lengths = _keep_books("fork", block_table, page_refs, cache_seqlens, page_size, rows, rows, parents)

@@ -116,6 +116,30 @@ def prepare_inter_sequence_metadata(
     return ops.prepare_inter_sequence_metadata(cu_seqlens_q, cu_seqlens_k, visibility_bits)
 
 
+def flash_attn_sink_func(
+    q: Tensor, k: Tensor, v: Tensor, sink_size: int, softmax_scale: float | None = None, causal: bool = False,
+    window_size: tuple[int, int] = (-1, -1), deterministic: bool = False, return_attn_probs: bool = False,
+) -> Tensor | tuple[Tensor, Tensor]:
+    """flash_attn_func with a sliding window whose first `sink_size` keys stay visible: query row i sees key j when the
+    right bound (or `causal`) allows it and j is within window_size[0] of it or below sink_size. Head dims 64, 72, 96 and
+    128, forward and backward. Keys and values that no row sees still have to be finite."""
+    from ._impl import ops
+
+    return ops.FlashAttnSinkFunc.apply(q, k, v, None, None, sink_size, softmax_scale, causal, window_size, deterministic, return_attn_probs)
+
+
+def flash_attn_varlen_sink_func(
+    q: Tensor, k: Tensor, v: Tensor, cu_seqlens_q: Tensor, cu_seqlens_k: Tensor, max_seqlen_q: int, max_seqlen_k: int,
+    sink_size: int, softmax_scale: float | None = None, causal: bool = False, window_size: tuple[int, int] = (-1, -1),
+    deterministic: bool = False, return_attn_probs: bool = False,
+) -> Tensor | tuple[Tensor, Tensor]:
+    """flash_attn_sink_func for packed batches (flash_attn_varlen_func): the first `sink_size` keys of every sequence stay
+    visible to its own rows. Rows behind the last sequence are neither read nor written, whatever they hold."""
+    from ._impl import ops
+
+    return ops.FlashAttnSinkFunc.apply(q, k, v, cu_seqlens_q, cu_seqlens_k, sink_size, softmax_scale, causal, window_size, deterministic, return_attn_probs)
+
+
 def flash_attn_paged_func(
     q: Tensor, k_cache: Tensor, v_cache: Tensor, block_table: Tensor, cache_seqlens: Tensor,
     softmax_scale: float | None = None, window_size: tuple[int, int] = (-1, -1), sink_size: int = 0,
@@ -216,8 +240,10 @@ __all__ = [
     "flash_attn_kvpacked_func",
     "flash_attn_paged_func",
     "flash_attn_qkvpacked_func",
+    "flash_attn_sink_func",
     "flash_attn_varlen_func",
     "flash_attn_varlen_kvpacked_func",
+    "flash_attn_varlen_sink_func",
     "fork_kv_pages",
     "free_kv_pages",
     "prepare_inter_sequence_metadata",
