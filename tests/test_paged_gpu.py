@@ -178,22 +178,24 @@ def test_decode_repeats_bit_for_bit_on_streams_and_in_graphs():
     torch.cuda.synchronize()
     for out, lse in got:
         assert torch.equal(out, want[0]) and torch.equal(lse, want[1])
-    # two graphs in one pool: each captured call has its own workspace, and replays read the tensors as they are then
-    pool = torch.cuda.graph_pool_handle()
-    graphs, results = [], []
-    for _ in range(2):
-        graph = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(graph, pool=pool):
-            results.append(call())
-        graphs.append(graph)
-    held.copy_(ints([2999, 18, 850, 5]))
-    table[3, 0] = table[0, 4]
-    want = call()
-    for graph in (*graphs, *reversed(graphs)):
-        graph.replay()
-    torch.cuda.synchronize()
-    for out, lse in results:
-        assert torch.equal(out, want[0]) and torch.equal(lse, want[1])
+    # Graphs with pools of their own may be replayed in any order, each with a workspace that nobody else writes; graphs
+    # that share a pool in the order of their capture (torch hands the second one the memory that the first has freed).
+    # Replays read the tensors as they are then.
+    for pool, order in ((None, (0, 1, 1, 0)), (torch.cuda.graph_pool_handle(), (0, 1, 0, 1))):
+        graphs, results = [], []
+        for _ in range(2):
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, pool=pool):
+                results.append(call())
+            graphs.append(graph)
+        held.copy_(ints([2999, 18, 850, 5] if pool is None else [1, 300, 2, 9]))
+        table[3, 0], table[1] = table[0, 4], table[0].flip(0)
+        want = call()
+        for i in order:
+            graphs[i].replay()
+        torch.cuda.synchronize()
+        for out, lse in results:
+            assert torch.equal(out, want[0]) and torch.equal(lse, want[1])
     torch.cuda.set_sync_debug_mode("error")
     try:
         call()
