@@ -13,13 +13,18 @@
 //     on the N side, where 8 (NT = 1), 16 or 32 of them cost no padding on the streamed operand.
 //   - A dot product does not care about the order of its terms, and neither does the order of the output columns matter
 //     until they are stored. Both are permuted so that what one thread needs of K and of V for its fragments is whole
-//     16-byte pieces: a thread copies its own pieces with cp.async into its own places of a ring in shared memory and
-//     reads them back itself. No transposition, no ldmatrix, no bank conflicts, no synchronisation.
+//     16-byte pieces: no transposition and no ldmatrix.
+//   - Each warp has a ring of its own in shared memory, filled by TMA boxes of 64 columns and 16 or 8 keys (pages whose
+//     size is a multiple of 8), its lane 0 issuing. Other page sizes are copied row by row with cp.async, every thread
+//     into places that it alone reads back; that stops at 4.1 to 4.7 TB/s, whatever
+//     is computed next to it.
 //   - The maximum of a column moves only when a score exceeds it by more than 8 (in log2 units), so a step costs one vote
 //     instead of a reduction over the lanes. Sums are kept per lane and added up at the end.
-// The steps of all sequences are dealt out in shares of equal size, so that long and short sequences keep every SM busy;
-// each block works out from the lengths which share it has. A sequence with one share is finished in place, the shares of
-// the others are joined by a second kernel.
+// The grid is one wave of blocks, and the steps of all (key head, sequence) pairs, laid end to end, are cut into as many
+// equal ranges: every SM is busy until the end however uneven the lengths are. (Shares per sequence, dealt out as whole
+// blocks, left the SMs idle a quarter of the time: 235 us instead of 173 us for 64 sequences of 100 to 8192 tokens.) A
+// block derives its range from the lengths. Pairs that lie within one range are finished in place; of a pair that is cut,
+// every range leaves a part, and a second kernel joins them.
 #include "common.h"
 #include "fwd_common.cuh"
 #include "paged_index.h"
@@ -30,7 +35,7 @@ namespace b200fa {
 struct PagedParams {
   int batch, heads_q, heads_kv, group, head_dim, num_pages, capacity, window_left, sink;
   FastDiv page_size, chunks;  // chunks of 8 * NT query heads per key head
-  int min_steps, target;      // shares: at least so many steps, about so many per (key head, chunk)
+  int columns, ranges;        // chunks of all key heads; ranges = blocks
   float scale_log2;
   const __nv_bfloat16* q;
   const __nv_bfloat16* k;
@@ -39,8 +44,12 @@ struct PagedParams {
   const int32_t* lengths;
   __nv_bfloat16* out;
   float* lse;
-  float* o_part;    // (slots, heads_q, head_dim): sum of p V relative to the share's maximum
-  float2* ml_part;  // (slots, heads_q): maximum (log2 units) and sum of p
+  // Parts of cut pairs, two slots per range: 2 r + 1 for the pair that begins in range r, 2 r for one that began before.
+  float* o_part;    // (slots, 8 * NT, head_dim): sum of p V relative to the part's maximum
+  float2* ml_part;  // (slots, 8 * NT): maximum (log2 units) and sum of p
+  int4* cut;        // (ranges): of the pair that the range begins inside of (sequence, chunk, first range, last range)
+  int box_rows;     // keys per TMA box: 16 or 8
+  int* status;      // device status word of the library (bounded waits)
   int64_t q_seq, q_head, k_page, k_row, k_head, v_page, v_row, v_head, out_seq, out_head, table_seq;
 };
 
@@ -70,375 +79,465 @@ __device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
 }
 __device__ __forceinline__ uint32_t word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
 
+// Four columns of an output row from their sums, and the row's log-sum-exp.
+__device__ __forceinline__ void store_output(const PagedParams& p, int b, int head, int d, float4 sum, float top, float total) {
+  const float inv = total > 0.f ? 1.f / total : 0.f;
+  *reinterpret_cast<uint2*>(p.out + b * p.out_seq + head * p.out_head + d) =
+      make_uint2(pack_bf16x2(sum.x * inv, sum.y * inv), pack_bf16x2(sum.z * inv, sum.w * inv));
+  if (d == 0) p.lse[(int64_t)b * p.heads_q + head] = total > 0.f ? (top + log2f(total)) * 0.69314718055994531f : -INFINITY;
+}
+
 // ---------------------------------------------------------------------------------------------- dealing out the steps
-// All blocks (of both kernels) derive the same plan from the lengths: with T steps in all, a share has
-// max(min_steps, ceil(T / target)) steps, so there are at most target + batch shares.
-struct PagedPlan {
-  int64_t share_steps;
-  __device__ __forceinline__ int shares(int steps) const {
-    return imax(1, (int)((steps + share_steps - 1) / share_steps));
+constexpr int kMinSteps = 6;  // a range has so many steps at least: one per warp at head_dim up to 128
+
+// A sequence without visible keys still has one (empty) step, in which its zeros are written.
+__device__ __forceinline__ int steps_of(const PagedParams& p, int b) {
+  return imax(1, paged_range(p.lengths[b], p.capacity, p.window_left, p.sink).steps);
+}
+
+// Block-wide exclusive prefix sum; adds the block's sum to *total.
+template <int kThreads>
+__device__ __forceinline__ int64_t prefix_sum(int mine, int64_t* total, int64_t* warp_sums) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int64_t inclusive = mine;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int64_t other = __shfl_up_sync(0xffffffffu, inclusive, d);
+    if (lane >= d) inclusive += other;
+  }
+  __syncthreads();  // the sums of an earlier call have been read
+  if (lane == 31) warp_sums[warp] = inclusive;
+  __syncthreads();
+  int64_t before = *total;
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w) {
+    if (w < warp) before += warp_sums[w];
+    *total += warp_sums[w];
+  }
+  return before + inclusive - mine;
+}
+
+// Quotient of non-negative numbers; the 64-bit division is a subroutine of some hundred instructions.
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+  return ((a | b) >> 32) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b;
+}
+
+// `work` steps in `ranges` ranges whose sizes differ by one at most, the longer ones first.
+struct Deal {
+  int64_t work, base;
+  int ranges, longer;
+  __device__ __forceinline__ Deal(int64_t steps, int blocks) : work(steps) {
+    const int64_t wanted = quotient(steps + kMinSteps - 1, kMinSteps);
+    ranges = wanted < blocks ? (int)wanted : blocks;
+    base = quotient(steps, ranges);
+    longer = (int)(steps - base * ranges);
+  }
+  __device__ __forceinline__ int64_t start(int r) const { return base * r + imin(r, longer); }
+  __device__ __forceinline__ int owner(int64_t at) const {
+    const int64_t front = (base + 1) * longer;
+    return (int)(at < front ? quotient(at, base + 1) : longer + quotient(at - front, base));
   }
 };
 
-__device__ __forceinline__ PagedRange range_of(const PagedParams& p, int b) {
-  return paged_range(p.lengths[b], p.capacity, p.window_left, p.sink);
-}
-
-template <int kThreads>
-__device__ __forceinline__ PagedPlan make_plan(const PagedParams& p, int64_t* warp_sums) {
-  int64_t mine = 0;
-  for (int b = threadIdx.x; b < p.batch; b += kThreads) mine += range_of(p, b).steps;
-#pragma unroll
-  for (int d = 16; d > 0; d >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, d);
-  if ((threadIdx.x & 31) == 0) warp_sums[threadIdx.x >> 5] = mine;
-  __syncthreads();
-  int64_t total = 0;
-#pragma unroll
-  for (int w = 0; w < kThreads / 32; ++w) total += warp_sums[w];
-  const int64_t even = (total + p.target - 1) / p.target;
-  return {even > p.min_steps ? even : p.min_steps};
-}
-
-// Calls visit(b, first slot, shares) in the threads that own a sequence b, sequences in order, until `done` says so for
-// the whole block: first slot = shares of the sequences in front of b.
-template <int kThreads, typename Visit, typename Done>
-__device__ __forceinline__ void walk_plan(const PagedParams& p, const PagedPlan& plan, int* warp_sums, Visit visit, Done done) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int before = 0;
-  for (int base = 0; base < p.batch; base += kThreads) {
-    const int b = base + threadIdx.x;
-    const int mine = b < p.batch ? plan.shares(range_of(p, b).steps) : 0;
-    int inclusive = mine;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const int other = __shfl_up_sync(0xffffffffu, inclusive, d);
-      if (lane >= d) inclusive += other;
-    }
-    if (lane == 31) warp_sums[warp] = inclusive;
-    __syncthreads();
-    int total = 0, front = before;
-#pragma unroll
-    for (int w = 0; w < kThreads / 32; ++w) {
-      if (w < warp) front += warp_sums[w];
-      total += warp_sums[w];
-    }
-    if (b < p.batch) visit(b, front + inclusive - mine, mine);
-    before += total;
-    __syncthreads();  // what visit() wrote is visible; the sums may be overwritten
-    if (done(base + kThreads)) return;
-  }
-}
-
-// ---------------------------------------------------------------------------------------------- the shares
+// ---------------------------------------------------------------------------------------------- the ranges
 template <int D, int NT>
 struct PagedConfig {
-  static constexpr int kWarps = D <= 128 ? 4 : 2;
+  // Twelve warps per SM, each with two steps in its ring, read 6.4 TB/s on 64 sequences of 100 to 8192 tokens (head_dim
+  // 128); eight warps with three steps 6.2, four with six 5.4: what counts is how many warps refill at the same time.
+  // 32 query heads of head_dim 128 leave registers for eight warps; from head_dim 256 on the ring sets the number.
+  static constexpr int kWarps = D <= 128 ? (D == 128 && NT == 4 ? 4 : 6) : 3;
   static constexpr int kThreads = 32 * kWarps;
-  static constexpr int kStepBytes = 2 * kPagedStep * D * 2;             // K and V of a step
-  static constexpr int kStages = D == 64 ? 6 : 3;                       // steps of a warp in flight
-  static constexpr int kRingBytes = kWarps * kStages * kStepBytes;      // 96 KiB: two blocks per SM (head_dim 512: one)
+  static constexpr int kStepBytes = 2 * kPagedStep * D * 2;         // K and V of a step
+  static constexpr int kStages = D == 64 ? 4 : D == 128 && NT == 4 ? 3 : 2;
+  static constexpr int kRingBytes = kWarps * kStages * kStepBytes;  // 96 KiB (head_dim 512: 192 KiB)
   static constexpr int kColumns = 8 * NT;
-  static constexpr int kMergeBytes = kWarps * kColumns * (D * 4 + 8);   // over the ring, at the end
-  static constexpr int kSmemBytes = kRingBytes > kMergeBytes ? kRingBytes : kMergeBytes;
+  static constexpr int kMergeBytes = kWarps * kColumns * (D * 4 + 8);  // over the ring, at the end of a pair
+  static constexpr int kSmemBytes = (kRingBytes > kMergeBytes ? kRingBytes : kMergeBytes) + 1024;  // alignment slack
+  static constexpr int kBlocksPerSm = D <= 256 ? 2 : 1;
 };
 
-// kAligned: page_size is a multiple of 16, so the keys of a step lie in one page; otherwise each lane looks up a key.
-template <int D, int NT, bool kAligned>
-__global__ void __launch_bounds__(PagedConfig<D, NT>::kThreads) paged_decode_kernel(const __grid_constant__ PagedParams p) {
+// kTma: page_size is a multiple of 8 and the ring is filled by TMA; otherwise each lane copies its own pieces.
+template <int D, int NT, bool kTma>
+__global__ void __launch_bounds__(PagedConfig<D, NT>::kThreads, PagedConfig<D, NT>::kBlocksPerSm)
+paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                    const __grid_constant__ PagedParams p) {
   using Cfg = PagedConfig<D, NT>;
-  constexpr int kStages = Cfg::kStages;
-  extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ int64_t plan_sums[Cfg::kWarps];
-  __shared__ int scan_sums[Cfg::kWarps], found[3];
+  constexpr int kStages = Cfg::kStages, kThreads = Cfg::kThreads, kPanelBytes = kPagedStep * 128;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t barriers[Cfg::kWarps][kStages];
+  __shared__ int64_t warp_sums[Cfg::kWarps], found_first;
+  __shared__ int found, abort_word;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);  // swizzled boxes: 1024-byte pattern
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int slot = blockIdx.x, kv_head = p.chunks.div(blockIdx.y);
-  const int column0 = (blockIdx.y - kv_head * p.chunks.divisor) * Cfg::kColumns;
+  const WaitCtx wctx{&abort_word, p.status, nullptr};
+  if (kTma && threadIdx.x == 32) {
+    tma_prefetch_descriptor(&map_k);
+    tma_prefetch_descriptor(&map_v);
+  }
+  if (threadIdx.x == 0) {
+    abort_word = 0;
+    for (int i = 0; i < Cfg::kWarps * kStages; ++i) mbar_init(smem_u32(&barriers[0][0]) + 8 * i, 1);
+    fence_barrier_init();
+  }
 
-  if (threadIdx.x == 0) found[0] = -1;
-  const PagedPlan plan = make_plan<Cfg::kThreads>(p, plan_sums);
-  walk_plan<Cfg::kThreads>(
-      p, plan, scan_sums,
-      [&](int b, int first, int shares) {
-        if (slot >= first && slot < first + shares) {
-          found[0] = b;
-          found[1] = slot - first;
-          found[2] = shares;
-        }
-      },
-      [&](int) { return found[0] >= 0; });
-  const int b = found[0];
-  if (b < 0) return;
-  const int share = found[1], shares = found[2];
-  const PagedRange range = range_of(p, b);
-  const int begin = (int)((int64_t)range.steps * share / shares), end = (int)((int64_t)range.steps * (share + 1) / shares);
-  const int32_t* table = p.table + b * p.table_seq;
-  const __nv_bfloat16* k_head = p.k + kv_head * p.k_head;
-  const __nv_bfloat16* v_head = p.v + kv_head * p.v_head;
-  const uint32_t ring = smem_u32(smem) + warp * kStages * Cfg::kStepBytes + lane * 16;
-
-  // The table entry that the step with number v needs (of this lane's key when the pages are not aligned); -1: none.
-  auto look_up = [&](int v) -> int {
-    if (v >= end) return -1;
-    const int key = range.step_of(v) * kPagedStep + (kAligned ? 0 : lane & 15);
-    return key < range.len ? table[p.page_size.div(key)] : -1;
-  };
-  // Starts the copies of step v; returns the set of its keys that the token sees.
-  auto issue = [&](int v, int stage, int page) -> uint32_t {
-    const int step = range.step_of(v), key = step * kPagedStep + (lane & 15);
-    const bool ok = v < end && page >= 0 && page < p.num_pages && range.sees(key);
-    const uint32_t mask = __ballot_sync(0xffffffffu, ok) & 0xffffu;
-    if (mask != 0) {
-      const uint32_t at = ring + stage * Cfg::kStepBytes;
-      int64_t k_own, v_own = 0;  // aligned: of the step's first row, else of this lane's key
-      {
-        const int first = kAligned ? step * kPagedStep : key;
-        const int row = first - p.page_size.div(first) * (int)p.page_size.divisor;
-        const bool have = kAligned || ok;
-        k_own = have ? page * p.k_page + row * p.k_row : 0;
-        v_own = have ? page * p.v_page + row * p.v_row : 0;
-      }
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int key_of = g + 8 * i;
-        const __nv_bfloat16* row = k_head + 8 * t + (kAligned ? k_own + key_of * p.k_row : __shfl_sync(0xffffffffu, k_own, key_of));
-        const bool seen = (mask >> key_of) & 1u;
-#pragma unroll
-        for (int c = 0; c < D / 32; ++c) {
-          const bool inside = seen && 32 * c + 8 * t < p.head_dim;
-          cp_async_16(at + (i * (D / 32) + c) * 512, inside ? row + 32 * c : k_head, inside);
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int key_of = 2 * t + (i & 1) + 8 * (i >> 1);
-        const __nv_bfloat16* row = v_head + 8 * g + (kAligned ? v_own + key_of * p.v_row : __shfl_sync(0xffffffffu, v_own, key_of));
-        const bool seen = (mask >> key_of) & 1u;
-#pragma unroll
-        for (int c = 0; c < D / 64; ++c) {
-          const bool inside = seen && 64 * c + 8 * g < p.head_dim;
-          cp_async_16(at + (D / 16 + i * (D / 64) + c) * 512, inside ? row + 64 * c : v_head, inside);
-        }
+  // ---- this block's range: steps [position, last) of the pairs in the order (chunk, sequence, step)
+  int64_t round = 0, before = 0;  // steps of all sequences; of those in front of this thread's
+  int mine = 0;
+  for (int base = 0; base < p.batch; base += kThreads) {
+    const int b = base + threadIdx.x;
+    mine = b < p.batch ? steps_of(p, b) : 0;
+    before = prefix_sum<kThreads>(mine, &round, warp_sums);
+  }
+  const Deal deal(round * p.columns, p.ranges);
+  if (blockIdx.x >= deal.ranges) {
+    if (threadIdx.x == 0) p.cut[blockIdx.x] = make_int4(-1, 0, 0, 0);
+    return;
+  }
+  int64_t position = deal.start(blockIdx.x);
+  const int64_t last = deal.start(blockIdx.x + 1);
+  int chunk = (int)quotient(position, round);
+  {
+    const int64_t offset = position - chunk * round;
+    if (p.batch <= kThreads) {
+      if (before <= offset && offset < before + mine) found = threadIdx.x, found_first = before;
+    } else {
+      int64_t total = 0;
+      for (int base = 0; base < p.batch && total <= offset; base += kThreads) {
+        const int b = base + threadIdx.x;
+        mine = b < p.batch ? steps_of(p, b) : 0;
+        before = prefix_sum<kThreads>(mine, &total, warp_sums);
+        if (before <= offset && offset < before + mine) found = b, found_first = before;
       }
     }
-    cp_async_commit();
-    return mask;
-  };
+  }
+  __syncthreads();
+  int b = found;
+  int64_t pair_start = chunk * round + found_first;
 
-  // The first copies are on their way before the queries are read.
-  uint32_t masks[kStages];
-  int v_next = begin + warp, page_next = look_up(v_next);
-#pragma unroll
-  for (int i = 0; i < kStages - 1; ++i) {
-    const int page = page_next;
-    page_next = look_up(v_next + Cfg::kWarps);
-    masks[i] = issue(v_next, i, page);
-    v_next += Cfg::kWarps;
-  }
-  uint4 q[NT][D / 32];
-#pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    const int column = column0 + 8 * n + g;
-    const __nv_bfloat16* row = p.q + b * p.q_seq + (kv_head * p.group + column) * p.q_head + 8 * t;
-#pragma unroll
-    for (int c = 0; c < D / 32; ++c)
-      q[n][c] = column < p.group && 32 * c + 8 * t < p.head_dim ? *reinterpret_cast<const uint4*>(row + 32 * c) : make_uint4(0, 0, 0, 0);
-  }
-  // Of columns 8 n + 2 t + j: m the reference maximum (the same in the eight lanes of a column), l this lane's sum of p.
-  float m[NT][2], l[NT][2], o[NT][D / 64][4][4];
-#pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    m[n][0] = m[n][1] = -INFINITY;
-    l[n][0] = l[n][1] = 0.f;
-#pragma unroll
-    for (int c = 0; c < D / 64; ++c)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) o[n][c][j][0] = o[n][c][j][1] = o[n][c][j][2] = o[n][c][j][3] = 0.f;
-  }
+  const uint32_t ring = smem_u32(smem) + warp * kStages * Cfg::kStepBytes, bars = smem_u32(&barriers[warp][0]);
+  // Where this lane finds its pieces in the ring slot of a step. TMA: panels of 16 keys x 64 columns, 128 bytes a key, the
+  // 16-byte pieces of key r in the order of the 128-byte swizzle (piece ^ (r & 7)); keys 8 to 15 are 1024 bytes behind keys
+  // 0 to 7. Otherwise: the lane's own pieces one after the other, 512 bytes apart.
+  const uint32_t k_place = kTma ? g * 128 + ((t ^ g) << 4) : lane * 16;
+  const uint32_t v_place0 = kTma ? 2 * t * 128 + ((g ^ (2 * t)) << 4) : lane * 16;
+  const uint32_t v_place1 = (2 * t + 1) * 128 + ((g ^ (2 * t + 1)) << 4);
+  uint32_t parity = 0;  // bit s: parity of the next completion of the barrier of stage s
 
-  int stage = 0;
-  for (int v = begin + warp; v < end; v += Cfg::kWarps) {
-    cp_async_wait<kStages - 2>();
-    {
+  for (bool first_pair = true; position < last; first_pair = false) {
+    const int kv_head = p.chunks.div(chunk), column0 = (chunk - kv_head * (int)p.chunks.divisor) * Cfg::kColumns;
+    const PagedRange range = paged_range(p.lengths[b], p.capacity, p.window_left, p.sink);
+    const int pair_steps = imax(1, range.steps);
+    const int begin = (int)(position - pair_start);
+    const int end = last - pair_start < pair_steps ? (int)(last - pair_start) : pair_steps;
+    const bool whole = begin == 0 && end == pair_steps;
+    if (first_pair && threadIdx.x == 0)
+      p.cut[blockIdx.x] = begin == 0 ? make_int4(-1, 0, 0, 0)
+                                     : make_int4(b, chunk, deal.owner(pair_start), deal.owner(pair_start + pair_steps - 1));
+    const int32_t* table = p.table + b * p.table_seq;
+
+    // The table entry of this lane's key (lane & 15) of step v; -1: none.
+    auto look_up = [&](int v) -> int {
+      if (v >= end) return -1;
+      const int key = range.step_of(v) * kPagedStep + (lane & 15);
+      return key < range.len ? table[p.page_size.div(key)] : -1;
+    };
+    // Starts the copies of step v; returns the set of its keys that the token sees.
+    auto issue = [&](int v, int stage, int page) -> uint32_t {
+      const int step = range.step_of(v), key = step * kPagedStep + (lane & 15);
+      const bool ok = v < end && page >= 0 && page < p.num_pages && range.sees(key);
+      const uint32_t mask = __ballot_sync(0xffffffffu, ok) & 0xffffu;
+      const uint32_t at = ring + stage * Cfg::kStepBytes;
+      if constexpr (kTma) {
+        if (mask != 0) {
+          const uint32_t bar = bars + 8 * stage;
+          if (lane == 0) mbar_expect_tx(bar, Cfg::kStepBytes);
+          __syncwarp();
+          if (lane < kPagedStep && (lane & (p.box_rows - 1)) == 0) {
+            const int row = key - p.page_size.div(key) * (int)p.page_size.divisor;
+            const int from = page >= 0 && page < p.num_pages ? page : p.num_pages;  // out of range: the box is zeros
+#pragma unroll 1
+            for (int c = 0; c < D / 64; ++c) {
+              tma_load_4d(at + c * kPanelBytes + lane * 128, &map_k, bar, 64 * c, kv_head, row, from);
+              tma_load_4d(at + (D / 64 + c) * kPanelBytes + lane * 128, &map_v, bar, 64 * c, kv_head, row, from);
+            }
+          }
+        }
+      } else {
+        if (mask != 0) {
+          // 16-byte pieces 8 t of the K rows g and g + 8, pieces 8 g of the V rows 2 t, 2 t + 1, 2 t + 8 and 2 t + 9. Rows
+          // that are not seen and columns at and above head_dim become zeros without being read.
+          const int row = key - p.page_size.div(key) * (int)p.page_size.divisor;
+          const int64_t k_own = ok ? page * p.k_page + row * p.k_row : 0, v_own = ok ? page * p.v_page + row * p.v_row : 0;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const __nv_bfloat16* from = p.k + kv_head * p.k_head + 8 * t + __shfl_sync(0xffffffffu, k_own, g + 8 * i);
+            const bool seen = (mask >> (g + 8 * i)) & 1u;
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c) {
+              const bool inside = seen && 32 * c + 8 * t < p.head_dim;
+              cp_async_16(at + k_place + (i * (D / 32) + c) * 512, inside ? from + 32 * c : p.k, inside);
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int of = 2 * t + (i & 1) + 8 * (i >> 1);
+            const __nv_bfloat16* from = p.v + kv_head * p.v_head + 8 * g + __shfl_sync(0xffffffffu, v_own, of);
+            const bool seen = (mask >> of) & 1u;
+#pragma unroll
+            for (int c = 0; c < D / 64; ++c) {
+              const bool inside = seen && 64 * c + 8 * g < p.head_dim;
+              cp_async_16(at + v_place0 + (D / 16 + i * (D / 64) + c) * 512, inside ? from + 64 * c : p.v, inside);
+            }
+          }
+        }
+        cp_async_commit();
+      }
+      return mask;
+    };
+
+    // The first copies are on their way before the queries are read.
+    uint32_t masks[kStages];
+    int v_next = begin + warp, page_next = look_up(v_next);
+#pragma unroll
+    for (int i = 0; i < kStages; ++i) {
       const int page = page_next;
       page_next = look_up(v_next + Cfg::kWarps);
-      masks[kStages - 1] = issue(v_next, stage == 0 ? kStages - 1 : stage - 1, page);
+      masks[i] = issue(v_next, i, page);
       v_next += Cfg::kWarps;
     }
-    const uint32_t mask = masks[0];
+    uint4 q[NT][D / 32];
 #pragma unroll
-    for (int i = 0; i + 1 < kStages; ++i) masks[i] = masks[i + 1];
-    const uint32_t at = ring + stage * Cfg::kStepBytes;
-    stage = stage + 1 == kStages ? 0 : stage + 1;
-    if (mask == 0) continue;  // uniform over the warp: a step whose page is missing
-
-    float s[NT][4];
+    for (int n = 0; n < NT; ++n) {
+      const int column = column0 + 8 * n + g;
+      const __nv_bfloat16* row = p.q + b * p.q_seq + (kv_head * p.group + column) * p.q_head + 8 * t;
 #pragma unroll
-    for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
-#pragma unroll
-    for (int c = 0; c < D / 32; ++c) {
-      const uint4 low = ld_shared_u4(at + c * 512), high = ld_shared_u4(at + (D / 32 + c) * 512);  // keys g and g + 8
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        mma_16816(s[n], low.x, high.x, low.y, high.y, q[n][c].x, q[n][c].y);
-        mma_16816(s[n], low.z, high.z, low.w, high.w, q[n][c].z, q[n][c].w);
-      }
+      for (int c = 0; c < D / 32; ++c)
+        q[n][c] = column < p.group && 32 * c + 8 * t < p.head_dim ? *reinterpret_cast<const uint4*>(row + 32 * c) : make_uint4(0, 0, 0, 0);
     }
-    // Scores in log2 units; keys that are not seen get -inf whatever stands in their rows.
-    const bool seen_low = (mask >> g) & 1u, seen_high = (mask >> (g + 8)) & 1u;
-    bool grows = false;
+    // Of columns 8 n + 2 t + j: m the reference maximum (the same in the eight lanes of a column), l this lane's sum of p.
+    float m[NT][2], l[NT][2], o[NT][D / 64][4][4];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      m[n][0] = m[n][1] = -INFINITY;
+      l[n][0] = l[n][1] = 0.f;
+#pragma unroll
+      for (int c = 0; c < D / 64; ++c)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[n][c][j][0] = o[n][c][j][1] = o[n][c][j][2] = o[n][c][j][3] = 0.f;
+    }
+
+    int stage = 0;
+    for (int v = begin + warp; v < end; v += Cfg::kWarps) {
+      const uint32_t mask = masks[0], at = ring + stage * Cfg::kStepBytes;
+      if constexpr (!kTma) cp_async_wait<kStages - 1>();
+      if (mask != 0) {  // uniform over the warp; 0: a step whose page is missing
+        if constexpr (kTma) {
+          if (!mbar_wait_warp(bars + 8 * stage, (parity >> stage) & 1u, wctx, kWaitKvFull)) break;
+          parity ^= 1u << stage;
+          if (mask != 0xffffu) {
+            // Rows that are not seen may hold anything; their probabilities are 0, but 0 x NaN is not.
+            for (int i = lane; i < kPagedStep * (D / 8); i += 32) {
+              const int row = i & 15, piece = i >> 4;
+              if (!((mask >> row) & 1u)) st_shared_zero16(at + (D / 64 + (piece >> 3)) * kPanelBytes + row * 128 + (piece & 7) * 16);
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+          }
+        }
+        float s[NT][4];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {
+          // pieces 32 c + 8 t of keys g and g + 8
+          const uint32_t from = kTma ? at + (c >> 1) * kPanelBytes + (k_place ^ ((c & 1) << 6)) : at + k_place + c * 512;
+          const uint4 low = ld_shared_u4(from), high = ld_shared_u4(from + (kTma ? 1024 : D / 32 * 512));
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            mma_16816(s[n], low.x, high.x, low.y, high.y, q[n][c].x, q[n][c].y);
+            mma_16816(s[n], low.z, high.z, low.w, high.w, q[n][c].z, q[n][c].w);
+          }
+        }
+        // Scores in log2 units; keys that are not seen get -inf whatever stands in their rows.
+        const bool seen_low = (mask >> g) & 1u, seen_high = (mask >> (g + 8)) & 1u;
+        bool grows = false;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            s[n][j] = seen_low ? s[n][j] * p.scale_log2 : -INFINITY;
+            s[n][2 + j] = seen_high ? s[n][2 + j] * p.scale_log2 : -INFINITY;
+            grows |= fmaxf(s[n][j], s[n][2 + j]) > m[n][j] + 8.f;
+          }
+        if (__any_sync(0xffffffffu, grows)) {
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              float top = fmaxf(s[n][j], s[n][2 + j]);
+#pragma unroll
+              for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+              top = fmaxf(top, m[n][j]);
+              const float alpha = top == -INFINITY ? 1.f : ex2_approx(m[n][j] - top);
+              m[n][j] = top;
+              l[n][j] *= alpha;
+#pragma unroll
+              for (int c = 0; c < D / 64; ++c)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  o[n][c][i][j] *= alpha;
+                  o[n][c][i][2 + j] *= alpha;
+                }
+            }
+        }
+        uint32_t prob[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          const float m0 = m[n][0] == -INFINITY ? 0.f : m[n][0], m1 = m[n][1] == -INFINITY ? 0.f : m[n][1];
+          const float p00 = ex2_approx(s[n][0] - m0), p01 = ex2_approx(s[n][1] - m1);
+          const float p10 = ex2_approx(s[n][2] - m0), p11 = ex2_approx(s[n][3] - m1);
+          l[n][0] += p00 + p10;
+          l[n][1] += p01 + p11;
+          prob[n][0] = transpose_8x8(pack_bf16x2(p00, p01));  // rounded to BF16 for the product, not for the sum
+          prob[n][1] = transpose_8x8(pack_bf16x2(p10, p11));
+        }
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c) {
+          uint4 row[4];  // keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9; columns 64 c + 8 g to + 7
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            row[i] = ld_shared_u4(kTma ? at + (D / 64 + c) * kPanelBytes + ((i & 1) ? v_place1 : v_place0) + (i >> 1) * 1024
+                                       : at + v_place0 + (D / 16 + i * (D / 64) + c) * 512);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint32_t w0 = word(row[0], j), w1 = word(row[1], j), w2 = word(row[2], j), w3 = word(row[3], j);
+            const uint32_t a0 = __byte_perm(w0, w1, 0x5410), a1 = __byte_perm(w0, w1, 0x7632);
+            const uint32_t a2 = __byte_perm(w2, w3, 0x5410), a3 = __byte_perm(w2, w3, 0x7632);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) mma_16816(o[n][c][j], a0, a1, a2, a3, prob[n][0], prob[n][1]);
+          }
+        }
+      }
+      // The slot is free again: the copies of the step kStages further on go there.
+      __syncwarp();
+      const int page = page_next;
+      page_next = look_up(v_next + Cfg::kWarps);
+#pragma unroll
+      for (int i = 0; i + 1 < kStages; ++i) masks[i] = masks[i + 1];
+      masks[kStages - 1] = issue(v_next, stage, page);
+      v_next += Cfg::kWarps;
+      stage = stage + 1 == kStages ? 0 : stage + 1;
+    }
+
+    // ---- the warps' parts go over the ring (nobody reads copies any more) and are joined
+    if constexpr (!kTma) cp_async_wait<0>();
+    __syncthreads();
+    if (kTma && *wctx.abort_flag) {  // a wait ran out: give copies in flight time to land before the block goes
+      for (int i = 0; i < 50; ++i) __nanosleep(20000);
+      return;
+    }
+    float* parts = reinterpret_cast<float*>(smem);  // (warp, column, D), then (warp, column) pairs of m and l
+    float2* part_ml = reinterpret_cast<float2*>(parts + Cfg::kWarps * Cfg::kColumns * D);
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        s[n][j] = seen_low ? s[n][j] * p.scale_log2 : -INFINITY;
-        s[n][2 + j] = seen_high ? s[n][2 + j] * p.scale_log2 : -INFINITY;
-        grows |= fmaxf(s[n][j], s[n][2 + j]) > m[n][j] + 8.f;
+        float sum = l[n][j];
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+        const int column = warp * Cfg::kColumns + 8 * n + 2 * t + j;
+        if (g == 0) part_ml[column] = make_float2(m[n][j], sum);
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            *reinterpret_cast<float2*>(parts + column * D + 64 * c + 8 * g + 2 * i) = make_float2(o[n][c][i][j], o[n][c][i][2 + j]);
       }
-    if (__any_sync(0xffffffffu, grows)) {
+    __syncthreads();
+    const int columns = imin(Cfg::kColumns, p.group - column0);
+    constexpr int kQuads = D / 4;
+    for (int i = threadIdx.x; i < columns * kQuads; i += kThreads) {
+      const int column = i / kQuads, d = 4 * (i - column * kQuads);
+      if (d >= p.head_dim) continue;
+      float top = -INFINITY, total = 0.f;
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+      for (int w = 0; w < Cfg::kWarps; ++w) top = fmaxf(top, part_ml[w * Cfg::kColumns + column].x);
+      float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          float top = fmaxf(s[n][j], s[n][2 + j]);
-#pragma unroll
-          for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-          top = fmaxf(top, m[n][j]);
-          const float alpha = top == -INFINITY ? 1.f : ex2_approx(m[n][j] - top);
-          m[n][j] = top;
-          l[n][j] *= alpha;
-#pragma unroll
-          for (int c = 0; c < D / 64; ++c)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              o[n][c][i][j] *= alpha;
-              o[n][c][i][2 + j] *= alpha;
-            }
-        }
-    }
-    uint32_t prob[NT][2];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const float m0 = m[n][0] == -INFINITY ? 0.f : m[n][0], m1 = m[n][1] == -INFINITY ? 0.f : m[n][1];
-      const float p00 = ex2_approx(s[n][0] - m0), p01 = ex2_approx(s[n][1] - m1);
-      const float p10 = ex2_approx(s[n][2] - m0), p11 = ex2_approx(s[n][3] - m1);
-      l[n][0] += p00 + p10;
-      l[n][1] += p01 + p11;
-      prob[n][0] = transpose_8x8(pack_bf16x2(p00, p01));  // rounded to BF16 for the product, not for the sum
-      prob[n][1] = transpose_8x8(pack_bf16x2(p10, p11));
-    }
-#pragma unroll
-    for (int c = 0; c < D / 64; ++c) {
-      uint4 row[4];  // keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9; columns 64 c + 8 g to + 7
-#pragma unroll
-      for (int i = 0; i < 4; ++i) row[i] = ld_shared_u4(at + (D / 16 + i * (D / 64) + c) * 512);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint32_t w0 = word(row[0], j), w1 = word(row[1], j), w2 = word(row[2], j), w3 = word(row[3], j);
-        const uint32_t a0 = __byte_perm(w0, w1, 0x5410), a1 = __byte_perm(w0, w1, 0x7632);
-        const uint32_t a2 = __byte_perm(w2, w3, 0x5410), a3 = __byte_perm(w2, w3, 0x7632);
-#pragma unroll
-        for (int n = 0; n < NT; ++n) mma_16816(o[n][c][j], a0, a1, a2, a3, prob[n][0], prob[n][1]);
+      for (int w = 0; w < Cfg::kWarps; ++w) {
+        const float2 ml = part_ml[w * Cfg::kColumns + column];
+        const float weight = top == -INFINITY ? 0.f : ex2_approx(ml.x - top);
+        const float4 part = *reinterpret_cast<const float4*>(parts + (w * Cfg::kColumns + column) * D + d);
+        total += weight * ml.y;
+        sum.x += weight * part.x, sum.y += weight * part.y, sum.z += weight * part.z, sum.w += weight * part.w;
+      }
+      if (whole) {
+        store_output(p, b, kv_head * p.group + column0 + column, d, sum, top, total);
+      } else {
+        const int64_t slot = (2 * (int64_t)blockIdx.x + (begin == 0)) * Cfg::kColumns + column;
+        *reinterpret_cast<float4*>(p.o_part + slot * p.head_dim + d) = sum;
+        if (d == 0) p.ml_part[slot] = make_float2(top, total);
       }
     }
-  }
-
-  // ---- the warps' parts go over the ring (nobody reads copies any more) and are joined
-  cp_async_wait<0>();
-  __syncthreads();
-  float* parts = reinterpret_cast<float*>(smem);  // (warp, column, D), then (warp, column) pairs of m and l
-  float2* part_ml = reinterpret_cast<float2*>(parts + Cfg::kWarps * Cfg::kColumns * D);
-#pragma unroll
-  for (int n = 0; n < NT; ++n)
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      float sum = l[n][j];
-#pragma unroll
-      for (int d = 4; d < 32; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-      const int column = warp * Cfg::kColumns + 8 * n + 2 * t + j;
-      if (g == 0) part_ml[column] = make_float2(m[n][j], sum);
-#pragma unroll
-      for (int c = 0; c < D / 64; ++c)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          *reinterpret_cast<float2*>(parts + column * D + 64 * c + 8 * g + 2 * i) = make_float2(o[n][c][i][j], o[n][c][i][2 + j]);
-    }
-  __syncthreads();
-  const int columns = imin(Cfg::kColumns, p.group - column0);
-  constexpr int kQuads = D / 4;
-  for (int i = threadIdx.x; i < columns * kQuads; i += Cfg::kThreads) {
-    const int column = i / kQuads, d = 4 * (i - column * kQuads);
-    if (d >= p.head_dim) continue;
-    float top = -INFINITY, total = 0.f;
-#pragma unroll
-    for (int w = 0; w < Cfg::kWarps; ++w) top = fmaxf(top, part_ml[w * Cfg::kColumns + column].x);
-    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-    for (int w = 0; w < Cfg::kWarps; ++w) {
-      const float2 ml = part_ml[w * Cfg::kColumns + column];
-      const float weight = top == -INFINITY ? 0.f : ex2_approx(ml.x - top);
-      const float4 part = *reinterpret_cast<const float4*>(parts + (w * Cfg::kColumns + column) * D + d);
-      total += weight * ml.y;
-      sum.x += weight * part.x, sum.y += weight * part.y, sum.z += weight * part.z, sum.w += weight * part.w;
-    }
-    const int head = kv_head * p.group + column0 + column;
-    if (shares == 1) {
-      const float inv = total > 0.f ? 1.f / total : 0.f;
-      *reinterpret_cast<uint2*>(p.out + b * p.out_seq + head * p.out_head + d) =
-          make_uint2(pack_bf16x2(sum.x * inv, sum.y * inv), pack_bf16x2(sum.z * inv, sum.w * inv));
-      if (d == 0) p.lse[(int64_t)b * p.heads_q + head] = total > 0.f ? (top + log2f(total)) * 0.69314718055994531f : -INFINITY;
-    } else {
-      const int64_t at = (int64_t)slot * p.heads_q + head;
-      *reinterpret_cast<float4*>(p.o_part + at * p.head_dim + d) = sum;
-      if (d == 0) p.ml_part[at] = make_float2(top, total);
+    if constexpr (kTma) fence_proxy_async_smem();
+    __syncthreads();  // the ring is free for the copies of the next pair
+    position = pair_start = pair_start + end;
+    if (++b == p.batch) {
+      b = 0;
+      ++chunk;
     }
   }
 }
 
-// Joins the shares of a sequence that has more than one: out = sum w o / sum w l, w = exp2(m - max m), in the order of the
-// shares. One block per (sequence, key head); it starts while the last shares are still being computed and waits for them
-// behind its own walk over the lengths.
-constexpr int kJoinThreads = 128;
+// Joins the parts of the pairs that were cut: out = sum w o / sum w l, w = exp2(m - max m). One block per (range, query head
+// of a chunk); the one of the pair's second range does the work. Its threads form groups of one thread per four columns,
+// group i takes the parts i, i + groups, ... in this order, and the groups are joined in order at the end, so the result
+// does not depend on the schedule. The blocks start under the last ranges and wait for them.
+constexpr int kJoinThreads = 256;
 __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_constant__ PagedParams p) {
-  __shared__ int64_t plan_sums[kJoinThreads / 32];
-  __shared__ int scan_sums[kJoinThreads / 32], found[2];
-  const int b = blockIdx.x;
-  const PagedPlan plan = make_plan<kJoinThreads>(p, plan_sums);
-  walk_plan<kJoinThreads>(
-      p, plan, scan_sums,
-      [&](int seq, int first, int shares) {
-        if (seq == b) {
-          found[0] = first;
-          found[1] = shares;
-        }
-      },
-      [&](int walked) { return walked > b; });
-  const int first = found[0], shares = found[1];
-  if (shares == 1) return;
+  __shared__ float4 group_o[kJoinThreads];
+  __shared__ float2 group_ml[kJoinThreads];
+  const int quads = p.head_dim / 4, groups = kJoinThreads / quads, columns = gridDim.y;
+  const int group = threadIdx.x / quads, quad = threadIdx.x - group * quads, column = blockIdx.y, range = blockIdx.x + 1;
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int quads = p.head_dim / 4;
-  for (int i = threadIdx.x; i < p.group * quads; i += kJoinThreads) {
-    const int column = i / quads, d = 4 * (i - column * quads), head = blockIdx.y * p.group + column;
-    const float2* ml = p.ml_part + (int64_t)first * p.heads_q + head;
-    const float* part = p.o_part + ((int64_t)first * p.heads_q + head) * p.head_dim + d;
-    float top = -INFINITY, total = 0.f;
-    for (int s = 0; s < shares; ++s) top = fmaxf(top, ml[(int64_t)s * p.heads_q].x);
-    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (top != -INFINITY) {
+  const int4 cut = p.cut[range];  // sequence, chunk, first range, last range
+  if (cut.x < 0 || cut.z != range - 1) return;
+  const int kv_head = p.chunks.div(cut.y), column0 = (cut.y - kv_head * (int)p.chunks.divisor) * columns;
+  if (column0 + column >= p.group) return;
+  const int parts = cut.w - cut.z + 1;
+  auto slot_of = [&](int i) { return (2 * (int64_t)(cut.z + i) + (i == 0)) * columns + column; };
+  float top = -INFINITY, total = 0.f;
+  float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (group < groups) {
 #pragma unroll 4
-      for (int s = 0; s < shares; ++s) {
-        const float2 own = ml[(int64_t)s * p.heads_q];
-        const float4 o = *reinterpret_cast<const float4*>(part + (int64_t)s * p.heads_q * p.head_dim);
-        const float weight = ex2_approx(own.x - top);
-        total += weight * own.y;
-        sum.x += weight * o.x, sum.y += weight * o.y, sum.z += weight * o.z, sum.w += weight * o.w;
-      }
+    for (int i = group; i < parts; i += groups) {
+      const float2 own = p.ml_part[slot_of(i)];
+      const float4 o = reinterpret_cast<const float4*>(p.o_part + slot_of(i) * p.head_dim)[quad];
+      const float higher = fmaxf(top, own.x);
+      const float keep = higher == -INFINITY ? 0.f : ex2_approx(top - higher), take = higher == -INFINITY ? 0.f : ex2_approx(own.x - higher);
+      top = higher;
+      total = total * keep + own.y * take;
+      sum.x = sum.x * keep + o.x * take, sum.y = sum.y * keep + o.y * take;
+      sum.z = sum.z * keep + o.z * take, sum.w = sum.w * keep + o.w * take;
     }
-    const float inv = total > 0.f ? 1.f / total : 0.f;
-    *reinterpret_cast<uint2*>(p.out + b * p.out_seq + head * p.out_head + d) =
-        make_uint2(pack_bf16x2(sum.x * inv, sum.y * inv), pack_bf16x2(sum.z * inv, sum.w * inv));
-    if (d == 0) p.lse[(int64_t)b * p.heads_q + head] = total > 0.f ? (top + log2f(total)) * 0.69314718055994531f : -INFINITY;
   }
+  group_o[threadIdx.x] = sum;
+  group_ml[threadIdx.x] = make_float2(top, total);
+  __syncthreads();
+  if (threadIdx.x >= quads) return;
+  top = -INFINITY;
+  for (int i = 0; i < groups; ++i) top = fmaxf(top, group_ml[i * quads].x);
+  total = 0.f;
+  sum = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i = 0; i < groups; ++i) {
+    const float2 own = group_ml[i * quads];
+    const float4 o = group_o[i * quads + quad];
+    const float weight = top == -INFINITY ? 0.f : ex2_approx(own.x - top);
+    total += weight * own.y;
+    sum.x += weight * o.x, sum.y += weight * o.y, sum.z += weight * o.z, sum.w += weight * o.w;
+  }
+  store_output(p, cut.x, kv_head * p.group + column0 + column, 4 * quad, sum, top, total);
 }
 
 // ---------------------------------------------------------------------------------------------- host side
@@ -452,47 +551,49 @@ static int paged_tiles(int head_dim, int group) {
 }
 
 struct PagedShape {
-  int tiles, chunks, min_steps, target;
-  int64_t slots;  // shares of all sequences, at most
+  int tiles, chunks, ranges;
+  size_t o_bytes, ml_bytes, cut_bytes;
+  size_t total() const { return o_bytes + ml_bytes + cut_bytes; }
 };
 static PagedShape paged_shape(const b200fa_paged_args& a) {
   PagedShape s;
   const int group = a.heads_q / a.heads_kv;
   s.tiles = paged_tiles(a.head_dim, group);
   s.chunks = (group + 8 * s.tiles - 1) / (8 * s.tiles);
-  const int64_t columns = (int64_t)a.heads_kv * s.chunks;
-  s.min_steps = 8;
-  s.target = (int)imax(1, (int)((4 * kPagedSms + columns - 1) / columns));
   const int64_t most_steps = ((int64_t)a.max_pages * a.page_size + kPagedStep - 1) / kPagedStep + 1;
-  const int64_t each = (most_steps + s.min_steps - 1) / s.min_steps;  // shares of one sequence, at most
-  s.slots = each <= 1 ? a.batch : (each * a.batch < (int64_t)s.target + a.batch ? each * a.batch : (int64_t)s.target + a.batch);
+  const int blocks_per_sm = a.head_dim <= 256 ? 2 : 1;
+  const int64_t most_work = most_steps * a.batch * a.heads_kv * s.chunks, wanted = (most_work + kMinSteps - 1) / kMinSteps;
+  s.ranges = wanted < blocks_per_sm * kPagedSms ? (int)wanted : blocks_per_sm * kPagedSms;
+  const size_t slots = 2 * (size_t)s.ranges * 8 * s.tiles;
+  s.o_bytes = slots * a.head_dim * 4;
+  s.ml_bytes = slots * 8;
+  s.cut_bytes = (size_t)s.ranges * 16;
   return s;
 }
 
-template <int D, int NT, bool kAligned>
-static int launch_paged(const PagedParams& p, dim3 grid, cudaStream_t stream) {
+template <int D, int NT, bool kTma>
+static int launch_paged(const CUtensorMap (&maps)[2], const PagedParams& p, cudaStream_t stream) {
   using Cfg = PagedConfig<D, NT>;
   static bool set[64] = {false};
-  const int status = set_dynamic_smem_once(reinterpret_cast<const void*>(&paged_decode_kernel<D, NT, kAligned>), Cfg::kSmemBytes, set);
+  const int status = set_dynamic_smem_once(reinterpret_cast<const void*>(&paged_decode_kernel<D, NT, kTma>), Cfg::kSmemBytes, set);
   if (status != B200FA_OK) return status;
-  paged_decode_kernel<D, NT, kAligned><<<grid, Cfg::kThreads, Cfg::kSmemBytes, stream>>>(p);
+  paged_decode_kernel<D, NT, kTma><<<p.ranges, Cfg::kThreads, Cfg::kSmemBytes, stream>>>(maps[0], maps[1], p);
   return B200FA_OK;
 }
 
 template <int D, int NT>
-static int launch_paged(const PagedParams& p, dim3 grid, cudaStream_t stream) {
-  return p.page_size.divisor % kPagedStep == 0 ? launch_paged<D, NT, true>(p, grid, stream)
-                                               : launch_paged<D, NT, false>(p, grid, stream);
+static int launch_paged(const CUtensorMap (&maps)[2], const PagedParams& p, cudaStream_t stream) {
+  return p.box_rows ? launch_paged<D, NT, true>(maps, p, stream) : launch_paged<D, NT, false>(maps, p, stream);
 }
 
 template <int D>
-static int launch_paged(int tiles, const PagedParams& p, dim3 grid, cudaStream_t stream) {
-  if (tiles == 1) return launch_paged<D, 1>(p, grid, stream);
+static int launch_paged(int tiles, const CUtensorMap (&maps)[2], const PagedParams& p, cudaStream_t stream) {
+  if (tiles == 1) return launch_paged<D, 1>(maps, p, stream);
   if constexpr (D <= 256) {
-    if (tiles == 2) return launch_paged<D, 2>(p, grid, stream);
+    if (tiles == 2) return launch_paged<D, 2>(maps, p, stream);
   }
   if constexpr (D <= 128) {
-    if (tiles == 4) return launch_paged<D, 4>(p, grid, stream);
+    if (tiles == 4) return launch_paged<D, 4>(maps, p, stream);
   }
   set_error("no paged attention kernel for %d query tiles at head_dim %d", tiles, D);
   return B200FA_ERR_UNSUPPORTED;
@@ -529,50 +630,61 @@ static int validate_paged(const b200fa_paged_args* a) {
 }
 
 size_t b200fa_paged_decode_workspace_bytes(const b200fa_paged_args* a) {
-  if (a->batch <= 0 || a->heads_kv <= 0 || a->heads_q <= 0) return 0;
-  const PagedShape s = paged_shape(*a);
-  return s.slots <= a->batch ? 0 : (size_t)s.slots * a->heads_q * (a->head_dim * 4 + 8);
+  if (a->batch <= 0 || a->heads_kv <= 0 || a->heads_q < a->heads_kv || a->page_size <= 0 || a->max_pages < 0) return 0;
+  return paged_shape(*a).total();
 }
 
 int b200fa_paged_decode(const b200fa_paged_args* a, void* stream) {
   int status = validate_paged(a);
   if (status != B200FA_OK || a->batch == 0) return status;
   const PagedShape shape = paged_shape(*a);
-  const size_t needed = b200fa_paged_decode_workspace_bytes(a);
-  B200FA_REQUIRE(a->workspace_bytes >= needed && (needed == 0 || a->workspace), "paged attention workspace is too small: need %zu bytes", needed);
+  B200FA_REQUIRE(a->workspace && a->workspace_bytes >= shape.total(), "paged attention workspace is too small: need %zu bytes",
+                 shape.total());
   B200FA_REQUIRE(reinterpret_cast<uintptr_t>(a->workspace) % 16 == 0, "paged attention workspace must be 16-byte aligned");
-  const int64_t columns = (int64_t)a->heads_kv * shape.chunks;
-  B200FA_REQUIRE(columns < 65536 && a->heads_kv < 65536, "too many heads for one call");
   PagedParams p;
   p.batch = a->batch, p.heads_q = a->heads_q, p.heads_kv = a->heads_kv, p.group = a->heads_q / a->heads_kv;
   p.head_dim = a->head_dim, p.num_pages = a->num_pages, p.capacity = a->max_pages * a->page_size;
   p.window_left = a->window_left, p.sink = a->sink_size;
   p.page_size = FastDiv::make((uint32_t)a->page_size), p.chunks = FastDiv::make((uint32_t)shape.chunks);
-  p.min_steps = shape.min_steps, p.target = shape.target;
+  p.columns = a->heads_kv * shape.chunks, p.ranges = shape.ranges;
   p.scale_log2 = a->softmax_scale * 1.4426950408889634f;
   p.q = static_cast<const __nv_bfloat16*>(a->q), p.k = static_cast<const __nv_bfloat16*>(a->k_cache);
   p.v = static_cast<const __nv_bfloat16*>(a->v_cache), p.out = static_cast<__nv_bfloat16*>(a->out);
   p.table = a->block_table, p.lengths = a->cache_seqlens, p.lse = a->softmax_lse;
-  p.o_part = static_cast<float*>(a->workspace);
-  p.ml_part = reinterpret_cast<float2*>(p.o_part + (size_t)shape.slots * a->heads_q * a->head_dim);
+  uint8_t* workspace = static_cast<uint8_t*>(a->workspace);
+  p.o_part = reinterpret_cast<float*>(workspace);
+  p.ml_part = reinterpret_cast<float2*>(workspace + shape.o_bytes);
+  p.cut = reinterpret_cast<int4*>(workspace + shape.o_bytes + shape.ml_bytes);
   p.q_seq = a->q_stride[0], p.q_head = a->q_stride[1], p.out_seq = a->out_stride[0], p.out_head = a->out_stride[1];
   p.k_page = a->k_stride[0], p.k_row = a->k_stride[1], p.k_head = a->k_stride[2];
   p.v_page = a->v_stride[0], p.v_row = a->v_stride[1], p.v_head = a->v_stride[2];
   p.table_seq = a->table_stride;
-  const dim3 grid((unsigned)shape.slots, (unsigned)columns);
+  p.status = device_status_word();
+  if (!p.status) return B200FA_ERR_CUDA;
+  // Boxes must not reach over the end of a page: 16 or 8 keys where the page size is a multiple of that.
+  CUtensorMap maps[2] = {};
+  p.box_rows = a->num_pages == 0 ? 0 : a->page_size % 16 == 0 ? 16 : a->page_size % 8 == 0 ? 8 : 0;
+  if (p.box_rows) {
+    for (int i = 0; i < 2; ++i) {
+      const int64_t* stride = i ? a->v_stride : a->k_stride;
+      status = encode_tensor_map(&maps[i], i ? a->v_cache : a->k_cache, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a->head_dim,
+                                 a->heads_kv, a->page_size, a->num_pages, stride[2], stride[1], stride[0], 64, p.box_rows);
+      if (status != B200FA_OK) return status;
+    }
+  }
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  status = a->head_dim <= 64    ? launch_paged<64>(shape.tiles, p, grid, s)
-           : a->head_dim <= 128 ? launch_paged<128>(shape.tiles, p, grid, s)
-           : a->head_dim <= 256 ? launch_paged<256>(shape.tiles, p, grid, s)
-                                : launch_paged<512>(shape.tiles, p, grid, s);
+  status = a->head_dim <= 64    ? launch_paged<64>(shape.tiles, maps, p, s)
+           : a->head_dim <= 128 ? launch_paged<128>(shape.tiles, maps, p, s)
+           : a->head_dim <= 256 ? launch_paged<256>(shape.tiles, maps, p, s)
+                                : launch_paged<512>(shape.tiles, maps, p, s);
   if (status != B200FA_OK) return status;
   B200FA_CUDA_CHECK(cudaGetLastError());
-  if (needed > 0) {
+  if (shape.ranges > 1) {
     cudaLaunchAttribute attribute;
     attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attribute.val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t config = {};
-    config.gridDim = dim3((unsigned)a->batch, (unsigned)a->heads_kv);
+    config.gridDim = dim3((unsigned)shape.ranges - 1, 8u * shape.tiles);
     config.blockDim = dim3(kJoinThreads);
     config.stream = s;
     config.attrs = &attribute;
