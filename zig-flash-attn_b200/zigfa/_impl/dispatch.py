@@ -1,0 +1,76 @@
+"""Short way from the public functions to the C entries, for operators that are called once per layer and token.
+
+An operator is registered with the dispatcher (schema, CUDA implementation, fake implementation for tracing), but plain
+tensors in eager mode go straight to the implementation: the dispatcher's way through Python costs 6 us a call, and the
+wrapper of `torch.library.custom_op` several times that, more than the small kernels take. Argument structures are packed
+with `struct` (1 us for forty fields) in the layout of include/b200fa.h.
+"""
+from __future__ import annotations
+
+import ctypes
+import functools
+import struct
+
+import torch
+
+from . import lib as _lib
+
+_library = torch.library.Library("zigfa", "FRAGMENT")
+_PLAIN = (torch.Tensor, torch.nn.Parameter)
+_is_compiling = torch.compiler.is_compiling
+_modes = torch._C._len_torch_dispatch_stack
+
+PROBLEM = "8if7P"  # b200fa_problem
+PACK_FWD = struct.Struct(f"@{PROBLEM}5P14qPN").pack
+PACK_BWD = struct.Struct(f"@{PROBLEM}9P26qPN").pack
+PACK_PAGED = struct.Struct("@9if7P11qPN").pack
+KV_CACHE = "4i2P6q"
+PACK_KV_CACHE = struct.Struct(f"@{KV_CACHE}").pack
+PACK_APPEND = struct.Struct(f"@{KV_CACHE}2P6qq3Pq2i").pack
+PACK_PAGES = struct.Struct("@5iPq7PN").pack
+
+
+def define(schema, implementation, fake):
+    """Registers zigfa::<schema> and returns the function that the host layer calls."""
+    name = schema.split("(")[0]
+    _library.define(schema)
+    _library.impl(name, implementation, "CUDA")
+    torch.library.register_fake(f"zigfa::{name}", fake, lib=_library)
+    op = getattr(torch.ops.zigfa, name).default
+
+    @functools.wraps(implementation)
+    def call(*arguments):
+        first = arguments[0]
+        if type(first) in _PLAIN and first.is_cuda and not _is_compiling() and not _modes():
+            return implementation(*arguments)
+        return op(*arguments)  # traced, transformed, or without a kernel for the device
+
+    return call
+
+
+@functools.cache
+def entry(name, *arguments):
+    """The C function `name` taking a packed structure first, then `arguments`."""
+    function = ctypes.CFUNCTYPE(ctypes.c_int, ctypes.c_char_p, *arguments)((name, _lib.library()))
+    return function
+
+
+def on_device(index, function, *arguments):
+    """function(*arguments) with the device made current; raises what its status says."""
+    if torch._C._cuda_getDevice() == index:
+        status = function(*arguments)
+    else:
+        with torch.cuda.device(index):
+            status = function(*arguments)
+    if status:
+        _lib.check(status)
+
+
+stream_of = torch._C._cuda_getCurrentRawStream
+
+
+def refuse_gradients(what, *tensors):
+    if torch.is_grad_enabled():
+        for tensor in tensors:
+            if tensor.requires_grad:
+                raise NotImplementedError(f"{what} has no backward pass: call it under torch.no_grad()")

@@ -338,7 +338,7 @@ def _(*unused):
     return None
 
 
-# ---- sliding window with sinks
+# ---- checks of the paged and the sink functions
 def check_sink_size(sink_size):
     if not isinstance(sink_size, numbers.Integral):
         raise TypeError(f"sink_size must be an integer, got {type(sink_size).__name__}")
@@ -350,57 +350,6 @@ def check_same_device(reference, **tensors):
     for name, tensor in tensors.items():
         if tensor is not None and tensor.device != reference.device:
             raise ValueError(f"{name} is on {tensor.device}, but the first tensor of the call is on {reference.device}")
-
-
-@torch.library.custom_op("zigfa::sink_forward", mutates_args=(), device_types="cuda")
-def sink_forward(
-    q: torch.Tensor,
-    k: torch.Tensor,
-    v: torch.Tensor,
-    cu_seqlens_q: torch.Tensor | None,
-    cu_seqlens_k: torch.Tensor | None,
-    softmax_scale: float,
-    window_size_left: int,
-    window_size_right: int,
-    sink_size: int,
-) -> tuple[torch.Tensor, torch.Tensor]:
-    check_same_device(q, k=k, v=v, cu_seqlens_q=cu_seqlens_q, cu_seqlens_k=cu_seqlens_k)
-    check_sink_size(sink_size)
-    return forward_impl(q, k, v, cu_seqlens_q, cu_seqlens_k, softmax_scale, window_size_left, window_size_right, sink=sink_size)
-
-
-@sink_forward.register_fake
-def _(q, k, v, cu_seqlens_q, *unused):
-    return q.new_empty(q.shape), q.new_empty(lse_shape(q, cu_seqlens_q is not None), dtype=torch.float32)
-
-
-@torch.library.custom_op("zigfa::sink_backward", mutates_args=(), device_types="cuda")
-def sink_backward(
-    dout: torch.Tensor,
-    q: torch.Tensor,
-    k: torch.Tensor,
-    v: torch.Tensor,
-    out: torch.Tensor,
-    softmax_lse: torch.Tensor,
-    cu_seqlens_q: torch.Tensor | None,
-    cu_seqlens_k: torch.Tensor | None,
-    softmax_scale: float,
-    window_size_left: int,
-    window_size_right: int,
-    sink_size: int,
-) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    check_same_device(q, dout=dout)
-    dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
-    backward_into(
-        dout, q, k, v, out, softmax_lse, cu_seqlens_q, cu_seqlens_k, softmax_scale, window_size_left,
-        window_size_right, dq, dk, dv, sink=sink_size,
-    )
-    return dq, dk, dv
-
-
-@sink_backward.register_fake
-def _(dout, q, k, v, *unused):
-    return q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
 
 
 # ---- inter-sequence
@@ -702,31 +651,6 @@ class FlashAttnVarlenKVPackedFunc(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dout, *unused):
         return _kvpacked_backward(ctx, dout)
-
-
-class FlashAttnSinkFunc(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, v, cu_seqlens_q, cu_seqlens_k, sink_size, softmax_scale, causal, window_size, deterministic,
-                return_attn_probs):
-        reject_unsupported(deterministic=deterministic)
-        check_sink_size(sink_size)
-        left, right = window_size
-        require_window(left, right)
-        softmax_scale = default_softmax_scale(softmax_scale, q.shape[-1])
-        if not softmax_scale > 0:
-            raise ValueError(f"attention with sinks needs a positive softmax_scale, got {softmax_scale}")
-        options = (softmax_scale, left, 0 if causal else right, sink_size)
-        out, softmax_lse = sink_forward(q, k, v, cu_seqlens_q, cu_seqlens_k, *options)
-        ctx.save_for_backward(q, k, v, out, softmax_lse, cu_seqlens_q, cu_seqlens_k)
-        ctx.options = options
-        if not return_attn_probs:
-            return out
-        ctx.mark_non_differentiable(softmax_lse)
-        return out, softmax_lse
-
-    @staticmethod
-    def backward(ctx, dout, *unused):
-        return _pad(ctx, *sink_backward(dout, *ctx.saved_tensors, *ctx.options))
 
 
 def _inter_sequence_window(causal, window_size, window_sizes):

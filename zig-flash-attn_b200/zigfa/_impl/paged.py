@@ -2,25 +2,23 @@
 pages, for writing tokens into them, copying them, and keeping the books of which sequence holds which page.
 
 The checks look at shapes, types, strides and devices only; what stands in the integer tensors (lengths, page numbers)
-stays on the device and is bounds-checked by the kernels. Work is enqueued on the current stream of the tensors' device
-and never synchronises. The ops are defined straight on the dispatcher: a decoding step calls them once per layer, and
-the wrapper that `torch.library.custom_op` puts around a function costs more host time than the small kernels take.
+stays on the device and is bounds-checked by the kernels. Each operation tests the whole of its conditions in one expression
+and turns to the check that names the fault only when that fails. Work is enqueued on the current stream of the tensors'
+device and never synchronises.
 """
 from __future__ import annotations
+
+import ctypes
+import functools
 
 import torch
 
 from . import lib as _lib
 from . import ops
+from .dispatch import (PACK_APPEND, PACK_KV_CACHE, PACK_PAGED, PACK_PAGES, define, entry, on_device, refuse_gradients,
+                       stream_of)
 
-_library = torch.library.Library("zigfa", "FRAGMENT")
-
-
-def _define(schema, implementation, fake):
-    name = schema.split("(")[0]
-    _library.define(schema)
-    _library.impl(name, implementation, "CUDA")
-    torch.library.register_fake(f"zigfa::{name}", fake, lib=_library)
+BF16, INT32 = torch.bfloat16, torch.int32
 
 
 # ------------------------------------------------------------------------------------------------ validation
@@ -50,7 +48,7 @@ def check_cache(k_cache, v_cache):
 
 
 def check_page_size(page_size):
-    if not isinstance(page_size, int) or page_size < 1:
+    if not isinstance(page_size, int) or not 0 < page_size < 2**31:
         raise ValueError(f"page_size must be a positive integer, got {page_size!r}")
 
 
@@ -119,171 +117,239 @@ def _table_stride(block_table):
     return block_table.stride(0) if block_table.shape[0] > 1 else block_table.shape[1]
 
 
-def _kv_cache(k_cache, v_cache):
-    num_pages, page_size, heads, head_dim = k_cache.shape
-    return _lib.KvCache(num_pages, page_size, heads, head_dim, k_cache.data_ptr(), v_cache.data_ptr(),
-                        _lib.Stride3(*k_cache.stride()[:3]), _lib.Stride3(*v_cache.stride()[:3]))
+def _is_table(block_table):
+    return block_table.dtype is INT32 and block_table.dim() == 2 and (block_table.stride(1) == 1 or block_table.shape[1] <= 1)
 
 
-def paged_forward(q, k_cache, v_cache, block_table, cache_seqlens, softmax_scale, window_left, sink_size):
-    check_paged(q, k_cache, v_cache, block_table, cache_seqlens, window_left, sink_size)
-    q, cache_seqlens = ops.readable(q), cache_seqlens.contiguous()
-    batch, heads_q, head_dim = q.shape
-    num_pages, page_size, heads_kv, _ = k_cache.shape
-    out = torch.empty((batch, heads_q, head_dim), dtype=torch.bfloat16, device=q.device)
-    softmax_lse = torch.empty((batch, heads_q), dtype=torch.float32, device=q.device)
-    library = _lib.library()
-    args = _lib.PagedArgs(
-        batch, heads_q, heads_kv, head_dim, num_pages, page_size, block_table.shape[1], window_left, sink_size,
-        softmax_scale, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(),
-        cache_seqlens.data_ptr(), out.data_ptr(), softmax_lse.data_ptr(), _lib.Stride2(*q.stride()[:2]),
-        _lib.Stride3(*k_cache.stride()[:3]), _lib.Stride3(*v_cache.stride()[:3]), _lib.Stride2(*out.stride()[:2]),
-        _table_stride(block_table),
+def _is_vector(tensor, size):
+    return tensor.dtype is INT32 and tensor.shape == (size,)
+
+
+def _is_cache(k_cache, v_cache):
+    shape, k_stride, v_stride = k_cache.shape, k_cache.stride(), v_cache.stride()
+    return (
+        k_cache.dtype is BF16 and v_cache.dtype is BF16 and len(shape) == 4 and v_cache.shape == shape
+        and shape[1] > 0 and shape[2] > 0 and shape[3] > 0 and k_stride[3] == 1 == v_stride[3]
+        and not (k_stride[0] | k_stride[1] | k_stride[2] | v_stride[0] | v_stride[1] | v_stride[2]) & 7
+        and not (k_cache.data_ptr() | v_cache.data_ptr()) & 15
     )
-    with torch.cuda.device(q.device):
-        workspace = ops._workspace(library.b200fa_paged_decode_workspace_bytes(args), q.device)
-        args.workspace, args.workspace_bytes = workspace.data_ptr(), workspace.numel()
-        _lib.check(library.b200fa_paged_decode(args, ops._stream(q.device)))
+
+
+@functools.lru_cache(maxsize=4096)
+def _paged_workspace(batch, heads_q, heads_kv, head_dim, page_size, max_pages):
+    args = _lib.PagedArgs(batch=batch, heads_q=heads_q, heads_kv=heads_kv, head_dim=head_dim, page_size=page_size, max_pages=max_pages)
+    return _lib.library().b200fa_paged_decode_workspace_bytes(args)
+
+
+def _paged_forward(q, k_cache, v_cache, block_table, cache_seqlens, softmax_scale, window_left, sink_size):
+    shape, cache_shape, device = q.shape, k_cache.shape, q.get_device()
+    if not (
+        q.dtype is BF16 and len(shape) == 3 and _is_cache(k_cache, v_cache) and shape[2] == cache_shape[3]
+        and _is_table(block_table) and block_table.shape[0] == shape[0] and _is_vector(cache_seqlens, shape[0])
+        and device == k_cache.get_device() == v_cache.get_device() == block_table.get_device() == cache_seqlens.get_device()
+        and type(sink_size) is int and 0 <= sink_size < 2**31
+    ):
+        check_paged(q, k_cache, v_cache, block_table, cache_seqlens, window_left, sink_size)
+    batch, heads_q, head_dim = shape
+    num_pages, page_size, heads_kv, _ = cache_shape
+    max_pages = block_table.shape[1]
+    if not cache_seqlens.is_contiguous():
+        cache_seqlens = cache_seqlens.contiguous()
+    if not ops.kernel_ready(q):
+        q = q.clone(memory_format=torch.contiguous_format)
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    softmax_lse = q.new_empty((batch, heads_q), dtype=torch.float32)
+    nbytes = _paged_workspace(batch, heads_q, heads_kv, head_dim, page_size, max_pages)
+    workspace = q.new_empty((nbytes,), dtype=torch.uint8)
+    q_stride, k_stride, v_stride = q.stride(), k_cache.stride(), v_cache.stride()
+    packed = PACK_PAGED(
+        batch, heads_q, heads_kv, head_dim, num_pages, page_size, max_pages, window_left, sink_size, softmax_scale,
+        q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), cache_seqlens.data_ptr(), out.data_ptr(),
+        softmax_lse.data_ptr(), q_stride[0], q_stride[1], k_stride[0], k_stride[1], k_stride[2],
+        v_stride[0], v_stride[1], v_stride[2], heads_q * head_dim, head_dim, _table_stride(block_table),
+        workspace.data_ptr(), nbytes,
+    )
+    on_device(device, entry("b200fa_paged_decode", ctypes.c_void_p), packed, stream_of(device))
     return out, softmax_lse
 
 
-_define(
+paged_forward = define(
     "paged_forward(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_table, Tensor cache_seqlens, float softmax_scale, "
     "int window_left, int sink_size) -> (Tensor, Tensor)",
-    paged_forward,
+    _paged_forward,
     lambda q, *unused: (q.new_empty(q.shape), q.new_empty(q.shape[:2], dtype=torch.float32)),
 )
 
 
-def append_kv(k, v, k_cache, v_cache, block_table, cache_seqlens, cu_seqlens):
-    check_append(k, v, k_cache, v_cache, block_table, cache_seqlens, cu_seqlens)
-    k, v, cache_seqlens = ops.readable(k), ops.readable(v), cache_seqlens.contiguous()
-    packed = cu_seqlens is not None
-    cu_seqlens = ops._contiguous_int(cu_seqlens)
-    args = _lib.AppendArgs(
-        _kv_cache(k_cache, v_cache), k.data_ptr(), v.data_ptr(), _lib.strides3(k, packed), _lib.strides3(v, packed),
-        k.shape[0] if packed else k.shape[1], _lib.pointer(cu_seqlens), cache_seqlens.data_ptr(), block_table.data_ptr(),
-        _table_stride(block_table), cache_seqlens.shape[0], block_table.shape[1],
+def _append_kv(k, v, k_cache, v_cache, block_table, cache_seqlens, cu_seqlens):
+    packed, shape, device, batch = cu_seqlens is not None, k.shape, k.get_device(), cache_seqlens.shape[0] if cache_seqlens.dim() else 0
+    if not (
+        k.dtype is BF16 and v.dtype is BF16 and v.shape == shape and len(shape) == (3 if packed else 4)
+        and _is_cache(k_cache, v_cache) and shape[-2:] == k_cache.shape[-2:] and not shape[-1] & 7 and shape[-1] <= 1024
+        and _is_vector(cache_seqlens, batch) and _is_table(block_table) and block_table.shape[0] == batch
+        and (_is_vector(cu_seqlens, batch + 1) and cu_seqlens.get_device() == device if packed else shape[0] == batch)
+        and device == v.get_device() == k_cache.get_device() == v_cache.get_device() == block_table.get_device() == cache_seqlens.get_device()
+    ):
+        check_append(k, v, k_cache, v_cache, block_table, cache_seqlens, cu_seqlens)
+    k, v, cache_seqlens, cu_seqlens = ops.readable(k), ops.readable(v), ops._contiguous_int(cache_seqlens), ops._contiguous_int(cu_seqlens)
+    num_pages, page_size, heads, head_dim = k_cache.shape
+    arguments = PACK_APPEND(
+        num_pages, page_size, heads, head_dim, k_cache.data_ptr(), v_cache.data_ptr(), *k_cache.stride()[:3],
+        *v_cache.stride()[:3], k.data_ptr(), v.data_ptr(), *((0, *k.stride()[:2]) if packed else k.stride()[:3]),
+        *((0, *v.stride()[:2]) if packed else v.stride()[:3]), shape[0] if packed else shape[1],
+        cu_seqlens.data_ptr() if packed else 0, cache_seqlens.data_ptr(), block_table.data_ptr(), _table_stride(block_table),
+        batch, block_table.shape[1],
     )
-    with torch.cuda.device(k.device):
-        _lib.check(_lib.library().b200fa_append_kv(args, ops._stream(k.device)))
+    on_device(device, entry("b200fa_append_kv", ctypes.c_void_p), arguments, stream_of(device))
 
 
-_define(
+append_kv = define(
     "append_kv(Tensor k, Tensor v, Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor block_table, Tensor cache_seqlens, "
     "Tensor? cu_seqlens) -> ()",
-    append_kv,
+    _append_kv,
     lambda *unused: None,
 )
 
 
-def copy_pages(k_cache, v_cache, source_pages, target_pages):
-    check_copy(k_cache, v_cache, source_pages, target_pages)
-    source_pages, target_pages = source_pages.contiguous(), target_pages.contiguous()
-    with torch.cuda.device(k_cache.device):
-        _lib.check(_lib.library().b200fa_copy_pages(
-            _kv_cache(k_cache, v_cache), source_pages.data_ptr(), target_pages.data_ptr(), source_pages.shape[0],
-            ops._stream(k_cache.device)))
+def _copy_pages(k_cache, v_cache, source_pages, target_pages):
+    device, count = k_cache.get_device(), source_pages.numel()
+    if not (
+        _is_cache(k_cache, v_cache) and not k_cache.shape[3] & 7 and k_cache.shape[3] <= 1024 and _is_vector(source_pages, count)
+        and _is_vector(target_pages, count)
+        and device == v_cache.get_device() == source_pages.get_device() == target_pages.get_device()
+    ):
+        check_copy(k_cache, v_cache, source_pages, target_pages)
+    source_pages, target_pages = ops._contiguous_int(source_pages), ops._contiguous_int(target_pages)
+    cache = PACK_KV_CACHE(*k_cache.shape, k_cache.data_ptr(), v_cache.data_ptr(), *k_cache.stride()[:3], *v_cache.stride()[:3])
+    call = entry("b200fa_copy_pages", ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int32, ctypes.c_void_p)
+    on_device(device, call, cache, source_pages.data_ptr(), target_pages.data_ptr(), count, stream_of(device))
 
 
-_define(
+copy_pages = define(
     "copy_pages(Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor source_pages, Tensor target_pages) -> ()",
-    copy_pages,
+    _copy_pages,
     lambda *unused: None,
 )
 
 
-def _keep_books(name, block_table, page_refs, cache_seqlens, page_size, rows, pairs, *extra):
-    """Runs one of the bookkeeping calls; returns (block_table, page_refs, source_pages, target_pages)."""
+def _are_books(block_table, page_refs, *per_sequence):
+    sequences, device = block_table.shape[0] if block_table.dim() else 0, block_table.get_device()
+    return (
+        _is_table(block_table) and page_refs.dtype is INT32 and page_refs.dim() == 1 and page_refs.get_device() == device
+        and all(_is_vector(tensor, sequences) and tensor.get_device() == device for tensor in per_sequence)
+    )
+
+
+def _like(tensor):
+    return torch.empty_like(tensor, memory_format=torch.contiguous_format)
+
+
+def _keep_books(name, block_table, page_refs, cache_seqlens, page_size, table_out, source, target, *extra):
+    """Runs one of the bookkeeping calls; returns the new page_refs."""
     sequences, max_pages = block_table.shape
-    num_pages, device = page_refs.shape[0], block_table.device
-    page_refs = page_refs.contiguous()
-    cache_seqlens = ops._contiguous_int(cache_seqlens)
-    extra = [tensor.contiguous() for tensor in extra]
-
-    def ints(*shape):
-        return torch.empty(shape, dtype=torch.int32, device=device)
-
-    table_out, refs_out = ints(rows, max_pages), ints(num_pages)
-    source, target = (ints(pairs), ints(pairs)) if pairs is not None else (None, None)
-    outputs = [ints(rows)] if name == "fork" else []
-    library = _lib.library()
-    nbytes = 0 if name == "free" else library.b200fa_pages_workspace_bytes(num_pages)
-    with torch.cuda.device(device):
-        workspace = ops._workspace(nbytes, device)
-        args = _lib.PagesArgs(
-            sequences, rows, max_pages, num_pages, page_size, block_table.data_ptr(), _table_stride(block_table),
-            page_refs.data_ptr(), _lib.pointer(cache_seqlens), table_out.data_ptr(), refs_out.data_ptr(),
-            _lib.pointer(source), _lib.pointer(target), workspace.data_ptr(), nbytes,
-        )
-        function = getattr(library, f"b200fa_{name}_pages")
-        _lib.check(function(args, *(tensor.data_ptr() for tensor in (*extra, *outputs)), ops._stream(device)))
-    return table_out, refs_out, source, target, *outputs
+    num_pages, device = page_refs.shape[0], block_table.get_device()
+    page_refs = ops._contiguous_int(page_refs)
+    refs_out = _like(page_refs)
+    scratch = None if name == "free" else _like(page_refs)
+    arguments = PACK_PAGES(
+        sequences, table_out.shape[0], max_pages, num_pages, page_size, block_table.data_ptr(), _table_stride(block_table),
+        page_refs.data_ptr(), 0 if cache_seqlens is None else cache_seqlens.data_ptr(), table_out.data_ptr(), refs_out.data_ptr(),
+        0 if source is None else source.data_ptr(), 0 if target is None else target.data_ptr(),
+        0 if scratch is None else scratch.data_ptr(), 0 if scratch is None else 4 * num_pages,
+    )
+    call = entry(f"b200fa_{name}_pages", *([ctypes.c_void_p] * (len(extra) + 1)))
+    on_device(device, call, arguments, *(tensor.data_ptr() for tensor in extra), stream_of(device))
+    return refs_out
 
 
-def reserve_pages(block_table, cache_seqlens, new_tokens, page_refs, page_size):
-    check_books(block_table, page_refs, cache_seqlens=cache_seqlens, new_tokens=new_tokens)
-    check_page_size(page_size)
-    return _keep_books("reserve", block_table, page_refs, cache_seqlens, page_size, block_table.shape[0], None, new_tokens)[:2]
+def _reserve_pages(block_table, cache_seqlens, new_tokens, page_refs, page_size):
+    if not (_are_books(block_table, page_refs, cache_seqlens, new_tokens) and type(page_size) is int and page_size > 0):
+        check_books(block_table, page_refs, cache_seqlens=cache_seqlens, new_tokens=new_tokens)
+        check_page_size(page_size)
+    table = _like(block_table)
+    refs = _keep_books("reserve", block_table, page_refs, ops._contiguous_int(cache_seqlens), page_size, table, None, None,
+                       ops._contiguous_int(new_tokens))
+    return table, refs
 
 
-def fork_pages(block_table, cache_seqlens, page_refs, parents, page_size):
-    check_books(block_table, page_refs, cache_seqlens=cache_seqlens)
-    check_ints("parents", parents, None)
-    ops.check_same_device(block_table, parents=parents)
-    check_page_size(page_size)
-    rows = parents.shape[0]
-    table, refs, source, target, lengths = _keep_books("fork", block_table, page_refs, cache_seqlens, page_size, rows, rows, parents)
+def _fork_pages(block_table, cache_seqlens, page_refs, parents, page_size):
+    if not (
+        _are_books(block_table, page_refs, cache_seqlens) and type(page_size) is int and page_size > 0
+        and _is_vector(parents, parents.numel()) and parents.get_device() == block_table.get_device()
+    ):
+        check_books(block_table, page_refs, cache_seqlens=cache_seqlens)
+        check_ints("parents", parents, None)
+        ops.check_same_device(block_table, parents=parents)
+        check_page_size(page_size)
+    table = block_table.new_empty((parents.shape[0], block_table.shape[1]))
+    parents = ops._contiguous_int(parents)
+    lengths, source, target = _like(parents), _like(parents), _like(parents)
+    refs = _keep_books("fork", block_table, page_refs, ops._contiguous_int(cache_seqlens), page_size, table, source, target,
+                       parents, lengths)
     return table, lengths, refs, source, target
 
 
-def free_pages(block_table, page_refs, first_entry, last_entry):
-    check_books(block_table, page_refs, first_entry=first_entry, last_entry=last_entry)
-    return _keep_books("free", block_table, page_refs, None, 1, block_table.shape[0], None, first_entry, last_entry)[:2]
+def _free_pages(block_table, page_refs, first_entry, last_entry):
+    if not _are_books(block_table, page_refs, first_entry, last_entry):
+        check_books(block_table, page_refs, first_entry=first_entry, last_entry=last_entry)
+    table = _like(block_table)
+    refs = _keep_books("free", block_table, page_refs, None, 1, table, None, None, ops._contiguous_int(first_entry),
+                       ops._contiguous_int(last_entry))
+    return table, refs
 
 
-def compact_pages(block_table, page_refs):
-    check_books(block_table, page_refs)
-    return _keep_books("compact", block_table, page_refs, None, 1, block_table.shape[0], page_refs.shape[0] // 2)
+def _compact_pages(block_table, page_refs):
+    if not _are_books(block_table, page_refs):
+        check_books(block_table, page_refs)
+    table, pairs = _like(block_table), (page_refs.shape[0] // 2,)
+    source, target = page_refs.new_empty(pairs), page_refs.new_empty(pairs)
+    refs = _keep_books("compact", block_table, page_refs, None, 1, table, source, target)
+    return table, refs, source, target
 
 
-def _like(table, *shape):
-    return table.new_empty(shape)
-
-
-_define(
+reserve_pages = define(
     "reserve_pages(Tensor block_table, Tensor cache_seqlens, Tensor new_tokens, Tensor page_refs, int page_size) -> (Tensor, Tensor)",
-    reserve_pages,
-    lambda table, lengths, new, refs, page_size: (_like(table, *table.shape), _like(refs, *refs.shape)),
+    _reserve_pages,
+    lambda table, lengths, new, refs, page_size: (table.new_empty(table.shape), refs.new_empty(refs.shape)),
 )
-_define(
+fork_pages = define(
     "fork_pages(Tensor block_table, Tensor cache_seqlens, Tensor page_refs, Tensor parents, int page_size) -> "
     "(Tensor, Tensor, Tensor, Tensor, Tensor)",
-    fork_pages,
+    _fork_pages,
     lambda table, lengths, refs, parents, page_size: (
-        _like(table, parents.shape[0], table.shape[1]), _like(parents, *parents.shape), _like(refs, *refs.shape),
-        _like(parents, *parents.shape), _like(parents, *parents.shape)),
+        table.new_empty((parents.shape[0], table.shape[1])), parents.new_empty(parents.shape), refs.new_empty(refs.shape),
+        parents.new_empty(parents.shape), parents.new_empty(parents.shape)),
 )
-_define(
+free_pages = define(
     "free_pages(Tensor block_table, Tensor page_refs, Tensor first_entry, Tensor last_entry) -> (Tensor, Tensor)",
-    free_pages,
-    lambda table, refs, *unused: (_like(table, *table.shape), _like(refs, *refs.shape)),
+    _free_pages,
+    lambda table, refs, *unused: (table.new_empty(table.shape), refs.new_empty(refs.shape)),
 )
-_define(
+compact_pages = define(
     "compact_pages(Tensor block_table, Tensor page_refs) -> (Tensor, Tensor, Tensor, Tensor)",
-    compact_pages,
-    lambda table, refs: (_like(table, *table.shape), _like(refs, *refs.shape), _like(refs, refs.shape[0] // 2),
-                         _like(refs, refs.shape[0] // 2)),
+    _compact_pages,
+    lambda table, refs: (table.new_empty(table.shape), refs.new_empty(refs.shape), refs.new_empty((refs.shape[0] // 2,)),
+                         refs.new_empty((refs.shape[0] // 2,))),
 )
 
 
 # ------------------------------------------------------------------------------------------------ public entry points
 def flash_attn_paged(q, k_cache, v_cache, block_table, cache_seqlens, softmax_scale, window_size, sink_size, return_lse):
     left, right = window_size
-    ops.require_window(left, right)
-    if torch.is_grad_enabled() and (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad):
-        raise NotImplementedError("paged attention has no backward pass: call it under torch.no_grad()")
+    if not (type(left) is int and type(right) is int and -1 <= left < 2**31 and right >= -1):
+        ops.require_window(left, right)
+        left = min(int(left), 2**31 - 1)
+    refuse_gradients("paged attention", q, k_cache, v_cache)
     softmax_scale = ops.default_softmax_scale(softmax_scale, q.shape[-1])
-    out, softmax_lse = torch.ops.zigfa.paged_forward(q, k_cache, v_cache, block_table, cache_seqlens, softmax_scale, left,
-                                                     sink_size)
-    return (out, softmax_lse) if return_lse else out
+    result = paged_forward(q, k_cache, v_cache, block_table, cache_seqlens, softmax_scale, left, sink_size)
+    return result if return_lse else result[0]
+
+
+def append_paged_kv(k, v, k_cache, v_cache, block_table, cache_seqlens, cu_seqlens):
+    refuse_gradients("writing into a cache", k, v, k_cache, v_cache)
+    append_kv(k, v, k_cache, v_cache, block_table, cache_seqlens, cu_seqlens)
+
+
+def copy_kv_pages(k_cache, v_cache, source_pages, target_pages):
+    refuse_gradients("copying pages", k_cache, v_cache)
+    copy_pages(k_cache, v_cache, source_pages, target_pages)

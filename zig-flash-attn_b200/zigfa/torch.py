@@ -123,9 +123,9 @@ def flash_attn_sink_func(
     """flash_attn_func with a sliding window whose first `sink_size` keys stay visible: query row i sees key j when the
     right bound (or `causal`) allows it and j is within window_size[0] of it or below sink_size. Head dims 64, 72, 96 and
     128, forward and backward. Keys and values that no row sees still have to be finite."""
-    from ._impl import ops
+    from ._impl import sink
 
-    return ops.FlashAttnSinkFunc.apply(q, k, v, None, None, sink_size, softmax_scale, causal, window_size, deterministic, return_attn_probs)
+    return sink.flash_attn_sink(q, k, v, None, None, sink_size, softmax_scale, causal, window_size, deterministic, return_attn_probs)
 
 
 def flash_attn_varlen_sink_func(
@@ -135,9 +135,9 @@ def flash_attn_varlen_sink_func(
 ) -> Tensor | tuple[Tensor, Tensor]:
     """flash_attn_sink_func for packed batches (flash_attn_varlen_func): the first `sink_size` keys of every sequence stay
     visible to its own rows. Rows behind the last sequence are neither read nor written, whatever they hold."""
-    from ._impl import ops
+    from ._impl import sink
 
-    return ops.FlashAttnSinkFunc.apply(q, k, v, cu_seqlens_q, cu_seqlens_k, sink_size, softmax_scale, causal, window_size, deterministic, return_attn_probs)
+    return sink.flash_attn_sink(q, k, v, cu_seqlens_q, cu_seqlens_k, sink_size, softmax_scale, causal, window_size, deterministic, return_attn_probs)
 
 
 def flash_attn_paged_func(
@@ -167,19 +167,17 @@ def append_paged_kv(
     k, v (sequences, tokens, heads_kv, head_dim), or packed (total, heads_kv, head_dim) with cu_seqlens (sequences + 1);
     token i of sequence b becomes key cache_seqlens[b] + i, so cache_seqlens counts the keys held before the call. Tokens
     whose table entry holds no page are dropped. Sequences must not share the pages that are written to."""
-    from ._impl import paged  # noqa: F401  registers the op
-    import torch
+    from ._impl import paged
 
-    torch.ops.zigfa.append_kv(k, v, k_cache, v_cache, block_table, cache_seqlens, cu_seqlens)
+    paged.append_paged_kv(k, v, k_cache, v_cache, block_table, cache_seqlens, cu_seqlens)
 
 
 def copy_kv_pages(k_cache: Tensor, v_cache: Tensor, source_pages: Tensor, target_pages: Tensor) -> None:
     """Copies page source_pages[i] of both caches to page target_pages[i], in place; a pair with an entry outside the cache
     (-1) is skipped. The targets must differ from one another and from every source."""
-    from ._impl import paged  # noqa: F401
-    import torch
+    from ._impl import paged
 
-    torch.ops.zigfa.copy_pages(k_cache, v_cache, source_pages, target_pages)
+    paged.copy_kv_pages(k_cache, v_cache, source_pages, target_pages)
 
 
 def reserve_kv_pages(
@@ -188,10 +186,9 @@ def reserve_kv_pages(
     """Pages for the next new_tokens[b] tokens of every sequence: the table entries behind those that cache_seqlens[b]
     tokens fill get a free page (page_refs <= 0) where they hold none, lowest pages first, in the order (sequence, entry);
     -1 stays where no page is left. Returns the new (block_table, page_refs)."""
-    from ._impl import paged  # noqa: F401
-    import torch
+    from ._impl import paged
 
-    return torch.ops.zigfa.reserve_pages(block_table, cache_seqlens, new_tokens, page_refs, page_size)
+    return paged.reserve_pages(block_table, cache_seqlens, new_tokens, page_refs, page_size)
 
 
 def fork_kv_pages(
@@ -201,10 +198,9 @@ def fork_kv_pages(
     whose page_refs count it, and gets a free page for the partly filled last one, to be copied in every layer with
     copy_kv_pages. Returns (child_table, child_seqlens, page_refs, source_pages, target_pages); a pair is -1 where nothing
     has to be copied or no page was left (the child's table entry is then -1 too)."""
-    from ._impl import paged  # noqa: F401
-    import torch
+    from ._impl import paged
 
-    return torch.ops.zigfa.fork_pages(block_table, cache_seqlens, page_refs, parents, page_size)
+    return paged.fork_pages(block_table, cache_seqlens, page_refs, parents, page_size)
 
 
 def free_kv_pages(
@@ -213,20 +209,18 @@ def free_kv_pages(
     """Gives the table entries [first_entry[b], last_entry[b]) of every sequence back: they become -1 and their pages lose
     a reference each; a page without references is free. Whole sequences (0 to max_pages) and pages that a window has left
     go the same way. Returns the new (block_table, page_refs)."""
-    from ._impl import paged  # noqa: F401
-    import torch
+    from ._impl import paged
 
-    return torch.ops.zigfa.free_pages(block_table, page_refs, first_entry, last_entry)
+    return paged.free_pages(block_table, page_refs, first_entry, last_entry)
 
 
 def compact_kv_pages(block_table: Tensor, page_refs: Tensor) -> tuple[Tensor, Tensor, Tensor, Tensor]:
     """Moves the pages in use to the front of the pool: with n of them, the i-th page in use at or behind n goes to the
     i-th free page in front of n. Returns the new (block_table, page_refs) and the pairs (source_pages, target_pages),
     -1 behind the last one, to be copied in every layer with copy_kv_pages."""
-    from ._impl import paged  # noqa: F401
-    import torch
+    from ._impl import paged
 
-    return torch.ops.zigfa.compact_pages(block_table, page_refs)
+    return paged.compact_pages(block_table, page_refs)
 
 
 __all__ = [
