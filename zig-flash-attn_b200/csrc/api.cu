@@ -130,7 +130,7 @@ long long* trace_buffer() { return g_trace.load(std::memory_order_relaxed); }
 
 int launch_fwd(const b200fa_fwd_args& args, int sink, cudaStream_t stream);
 int launch_bwd(const b200fa_bwd_args& args, int sink, cudaStream_t stream);
-size_t bwd_workspace_bytes(const b200fa_problem& problem);
+size_t bwd_workspace_bytes(const b200fa_problem& problem, int sink);
 void arm_bwd_timing(void* const* events);
 
 static int validate_problem(const b200fa_problem& p) {
@@ -240,9 +240,11 @@ int b200fa_bwd_timing_events(void* const* events) {
   return B200FA_OK;
 }
 
-size_t b200fa_bwd_workspace_bytes(const b200fa_problem* p) { return bwd_workspace_bytes(*p); }
+size_t b200fa_bwd_workspace_bytes(const b200fa_problem* p) { return bwd_workspace_bytes(*p, 0); }
 
-size_t b200fa_sink_bwd_workspace_bytes(const b200fa_problem* p, int32_t) { return bwd_workspace_bytes(*p); }
+size_t b200fa_sink_bwd_workspace_bytes(const b200fa_problem* p, int32_t sink_size) {
+  return bwd_workspace_bytes(*p, sinks_of(*p, sink_size));
+}
 
 int b200fa_bwd(const b200fa_bwd_args* args, void* stream) { return b200fa_sink_bwd(args, 0, stream); }
 

@@ -324,6 +324,12 @@ struct QueryCursorT {
     }
   }
 
+  // Keeps the blocks that start in rows [first, last), multiples of kBlockM (right after init; one run only).
+  B200FA_HD void restrict_to_rows(int first, int last) {
+    blk = imax(blk, first / kBlockM);
+    blk_end = imin(blk_end, last / kBlockM);
+  }
+
   B200FA_HD bool bit(int i) const {
     return (static_cast<uint32_t>(p->bits_t[seq * p->words + (i >> 5)]) >> (i & 31)) & 1u;
   }

@@ -86,18 +86,41 @@ bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CU
   using Cursor = QueryCursorT<!kSink, kSink>;
   const Problem& pr = p.prob;
   // ---- work item (uniform over the CTA; exits before any barrier or TMEM allocation)
-  int seq, n_block, kv_head;
-  if (p.work_list) {
-    const int2 e = p.work_list[blockIdx.x];
-    seq = e.x;
-    n_block = e.y;
-    kv_head = blockIdx.y;
-    if (seq >= pr.batch) return;
+  int seq, n_block, kv_head, share = -1;
+  if (kSink && blockIdx.x < p.sinks.ctas) {
+    // a share of a key block that holds sinks
+    const int entry = blockIdx.x / p.sinks.blocks;
+    n_block = blockIdx.x - entry * p.sinks.blocks;
+    if (p.sinks.list) {
+      const int2 e = p.sinks.list[entry];
+      seq = e.x;
+      share = e.y;
+      kv_head = blockIdx.y;
+      if (seq >= pr.batch) return;
+    } else {
+      const int pair = entry / p.sinks.per_sequence;
+      share = entry - pair * p.sinks.per_sequence;
+      seq = pair / pr.heads_kv;
+      kv_head = pair - seq * pr.heads_kv;
+    }
   } else {
-    const BwdCta cta = bwd_cta_of(p, blockIdx.x);
-    seq = cta.seq;
-    n_block = cta.n_block;
-    kv_head = cta.head_slot;
+    const int linear = kSink ? blockIdx.x - p.sinks.ctas : blockIdx.x;
+    if (p.work_list) {
+      const int2 e = p.work_list[linear];
+      seq = e.x;
+      n_block = e.y;
+      kv_head = blockIdx.y;
+      if (seq >= pr.batch) return;
+    } else {
+      const BwdCta cta = bwd_cta_of(p, linear);
+      seq = cta.seq;
+      n_block = cta.n_block;
+      kv_head = cta.head_slot;
+    }
+    if (kSink && p.sinks.rows) {
+      if (!p.work_list) n_block += p.sinks.blocks;  // the fixed-length launch leaves the blocks of the shares out
+      else if (n_block * kBlockN < pr.sink) return;
+    }
   }
   const SeqInfo s = seq_info(pr, seq);
   const int n0 = n_block * kBlockN;
@@ -105,6 +128,11 @@ bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CU
   const int c1 = imin(n0 + kBlockN, s.lk);
   const int group = pr.heads_q / pr.heads_kv;
   const int64_t stat_base = pr.cu_q ? 0 : (int64_t)seq * pr.seqlen_q;
+  // Walks the query blocks of this CTA: all that see the key block, or those of its share.
+  auto start_cursor = [&](Cursor& cur) {
+    cur.init(&pr, seq, s, n0, c1);
+    if (kSink && share >= 0) cur.restrict_to_rows(share * p.sinks.rows, (share + 1) * p.sinks.rows);
+  };
 
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   const uint32_t base = smem_u32(smem_raw);
@@ -163,7 +191,7 @@ bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CU
   int blocks_per_head = 0;
   {
     Cursor cur;
-    cur.init(&pr, seq, s, n0, c1);
+    start_cursor(cur);
     OtherBlock qb;
     while (cur.next(&qb)) ++blocks_per_head;
   }
@@ -193,7 +221,7 @@ bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CU
       const float* lse_head = p.lse_log2 + (int64_t)head * p.rows;
       const float* dpsum_head = p.dpsum + (int64_t)head * p.rows;
       Cursor cur;
-      cur.init(&pr, seq, s, n0, c1);
+      start_cursor(cur);
       OtherBlock qb;
       while (cur.next(&qb)) {
         const int st = it & 1;
@@ -343,7 +371,7 @@ bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CU
     bool ok = true;
     for (int g = 0; ok && g < group; ++g) {
       Cursor cur;
-      cur.init(&pr, seq, s, n0, c1);
+      start_cursor(cur);
       OtherBlock qb;
       while (cur.next(&qb)) {
         const int st = it & 1;
@@ -497,6 +525,12 @@ bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CU
         const int64_t hs = is_dv ? p.dv_head_stride : p.dk_head_stride;
         const float mul = is_dv ? 1.f : p.scale;
         const uint32_t t_acc = tmem_base + lane_addr + (is_dv ? Cfg::kTmemDv : Cfg::kTmemDk);
+        float* part_row = nullptr;  // a share leaves its sums in FP32, not scaled
+        if (kSink && share >= 0) {
+          const int64_t q0 = pr.cu_q ? s.q0 : (int64_t)seq * pr.seqlen_q;
+          const int64_t slot = q0 / p.sinks.rows + seq + share;
+          part_row = p.sinks.part + ((((slot * pr.heads_kv + kv_head) * p.sinks.blocks + n_block) * 2 + !is_dv) * kBlockN + r) * D;
+        }
         uint4* dst = reinterpret_cast<uint4*>(out + s.batch_coord * bs + (int64_t)(s.k0 + c) * rs + (int64_t)kv_head * hs);
 #pragma unroll
         for (int ch0 = 0; ch0 < D / 32 / kParts; ++ch0) {
@@ -509,7 +543,11 @@ bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CU
 #pragma unroll
             for (int i = 0; i < 32; ++i) acc[i] = 0;
           }
-          if (key_valid && p.dkv_wide) {  // 32-byte stores: a lane writes whole sectors of its row
+          if (kSink && part_row) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              reinterpret_cast<uint4*>(part_row + 32 * ch)[i] = make_uint4(acc[4 * i], acc[4 * i + 1], acc[4 * i + 2], acc[4 * i + 3]);
+          } else if (key_valid && p.dkv_wide) {  // 32-byte stores: a lane writes whole sectors of its row
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
               uint32_t w[8];
@@ -550,7 +588,7 @@ bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CU
     for (int g = 0; ok && g < group; ++g) {
       const int head = kv_head * group + g;
       Cursor cur;
-      cur.init(&pr, seq, s, n0, c1);
+      start_cursor(cur);
       OtherBlock qb;
       while (cur.next(&qb)) {
         const int row0 = (int)(stat_base + qb.row);
@@ -840,6 +878,38 @@ __global__ void __launch_bounds__(256) bwd_fix_dk_kernel(const float* __restrict
   }
 }
 
+// dK and dV of the key blocks whose work was dealt out in shares: the sum of the shares' parts, in their order. One block of
+// 256 threads per (key block of a sequence, key head, 256 / (D / 4) rows); a thread adds four columns of dV and of dK.
+template <int D>
+__global__ void __launch_bounds__(256) bwd_sink_join_kernel(const __grid_constant__ BwdParams p) {
+  constexpr int kQuads = D / 4, kRows = 256 / kQuads;
+  const Problem& pr = p.prob;
+  const int per_block = kBlockN / kRows;
+  const int group = blockIdx.x / per_block, r = (blockIdx.x - group * per_block) * kRows + threadIdx.x / kQuads;
+  const int seq = group / p.sinks.blocks, n_block = group - seq * p.sinks.blocks, kv_head = blockIdx.y;
+  const int column = 4 * (threadIdx.x % kQuads);
+  const SeqInfo s = seq_info(pr, seq);
+  const int c = n_block * kBlockN + r;
+  if (n_block * kBlockN >= pr.sink || c >= s.lk || column >= p.head_dim) return;
+  const int64_t q0 = pr.cu_q ? s.q0 : (int64_t)seq * pr.seqlen_q, slot0 = q0 / p.sinks.rows + seq;
+  const int shares = ceil_div(s.lq, p.sinks.rows);
+  const int64_t tile = (int64_t)kBlockN * D, stride = (int64_t)pr.heads_kv * p.sinks.blocks * 2 * tile;
+  const float* part = p.sinks.part + slot0 * stride + (((int64_t)kv_head * p.sinks.blocks + n_block) * 2) * tile + r * D + column;
+  float4 dv = make_float4(0.f, 0.f, 0.f, 0.f), dk = dv;
+#pragma unroll 4
+  for (int i = 0; i < shares; ++i) {
+    const float4 a = *reinterpret_cast<const float4*>(part + i * stride);
+    const float4 b = *reinterpret_cast<const float4*>(part + i * stride + tile);
+    dv.x += a.x, dv.y += a.y, dv.z += a.z, dv.w += a.w;
+    dk.x += b.x, dk.y += b.y, dk.z += b.z, dk.w += b.w;
+  }
+  const int64_t row = s.k0 + c;
+  *reinterpret_cast<uint2*>(p.dv + s.batch_coord * p.dv_batch_stride + row * p.dv_row_stride + kv_head * p.dv_head_stride + column) =
+      make_uint2(pack_bf16x2(dv.x, dv.y), pack_bf16x2(dv.z, dv.w));
+  *reinterpret_cast<uint2*>(p.dk + s.batch_coord * p.dk_batch_stride + row * p.dk_row_stride + kv_head * p.dk_head_stride + column) =
+      make_uint2(pack_bf16x2(dk.x * p.scale, dk.y * p.scale), pack_bf16x2(dk.z * p.scale, dk.w * p.scale));
+}
+
 // ---------------------------------------------------------------------------------------------- host side
 static thread_local cudaEvent_t g_timing_events[4];
 static thread_local bool g_timing_armed = false;
@@ -853,11 +923,30 @@ static void mark(int index, cudaStream_t stream) {
 }
 
 struct BwdWorkspace {
-  size_t lse_log2, dpsum, pivot_sum, pivot_key, dq_accum, dk_fix, dk_fix_bytes, work_list, total;
+  size_t lse_log2, dpsum, pivot_sum, pivot_key, dq_accum, dk_fix, dk_fix_bytes, work_list, sink_list, sink_part, total;
   int64_t rows, key_rows, entries;
+  int sink_rows, sink_blocks;     // SinkShares::rows and blocks
+  int64_t sink_entries;           // packed: entries of the shares' work list
 };
 
-static BwdWorkspace plan_workspace(const b200fa_problem& p) {
+// Query rows per share of the key blocks that hold sinks; 0: these blocks are not dealt out. A share should weigh about as
+// much as an ordinary key block (the window's query blocks), at most an eighth of what an SM has to do on average, so that
+// the launch ends evenly, and at least four query blocks, because a CTA has about two iterations' worth of set-up. Sinks that
+// fill more than four key blocks, windows without a right bound (whose key blocks are seen by half of the rows on average)
+// and sequences of less than two shares gain nothing.
+static int sink_share_rows(const b200fa_problem& p, int sink) {
+  if (sink <= 0 || sink > 4 * kBlockN || p.window_right < 0 || p.window_left < 0 || p.batch <= 0) return 0;
+  const bool packed = p.cu_seqlens_q != nullptr;
+  const int64_t row_blocks = ((packed ? 1 : (int64_t)p.batch) * p.seqlen_q + kBlockM - 1) / kBlockM;  // of all sequences
+  const int64_t window_blocks = ((int64_t)p.window_left + p.window_right + kBlockN) / kBlockM + 1;
+  const int64_t average = p.heads_kv * row_blocks * (window_blocks + ceil_div(sink, kBlockN)) / 148;
+  int64_t blocks = window_blocks > 4 ? window_blocks : 4;
+  if (blocks < average / 8) blocks = average / 8;
+  if (blocks * 2 * kBlockM > (int64_t)p.seqlen_q) return 0;  // (packed: no sequence can have two shares)
+  return (int)(blocks * kBlockM);
+}
+
+static BwdWorkspace plan_workspace(const b200fa_problem& p, int sink) {
   BwdWorkspace w;
   const bool packed = p.cu_seqlens_q != nullptr;
   w.rows = packed ? (int64_t)p.seqlen_q : (int64_t)p.batch * p.seqlen_q;
@@ -877,10 +966,21 @@ static BwdWorkspace plan_workspace(const b200fa_problem& p) {
   w.work_list = w.dk_fix + w.dk_fix_bytes;
   w.entries = packed ? work_list_entries(p.seqlen_k, p.batch, kBlockN) : 0;
   w.total = w.work_list + (size_t)w.entries * 8;
+  w.sink_rows = sink_share_rows(p, sink);
+  w.sink_blocks = w.sink_rows ? ceil_div(sink, kBlockN) : 0;
+  w.sink_entries = 0;
+  w.sink_list = w.sink_part = w.total;
+  if (w.sink_rows) {
+    w.sink_entries = packed ? work_list_entries(p.seqlen_q, p.batch, w.sink_rows) : 0;
+    w.sink_list = (w.total + 255) & ~size_t(255);
+    w.sink_part = (w.sink_list + (size_t)w.sink_entries * 8 + 255) & ~size_t(255);
+    const size_t slots = (size_t)(w.rows / w.sink_rows) + p.batch;
+    w.total = w.sink_part + slots * p.heads_kv * w.sink_blocks * 2 * kBlockN * compiled_dim * 4;
+  }
   return w;
 }
 
-size_t bwd_workspace_bytes(const b200fa_problem& p) { return plan_workspace(p).total; }
+size_t bwd_workspace_bytes(const b200fa_problem& p, int sink) { return plan_workspace(p, sink).total; }
 
 template <int D>
 static int launch_main(const b200fa_bwd_args& a, const BwdParams& p, dim3 grid, float* dq_accum, int64_t stat_rows,
@@ -942,7 +1042,7 @@ template <int D>
 static int launch_bwd_d(const b200fa_bwd_args& a, int sink, cudaStream_t stream) {
   const b200fa_problem& bp = a.problem;
   const bool packed = bp.cu_seqlens_q != nullptr;
-  const BwdWorkspace w = plan_workspace(bp);
+  const BwdWorkspace w = plan_workspace(bp, sink);
   B200FA_REQUIRE(a.workspace_bytes >= w.total && (w.total == 0 || a.workspace), "backward workspace is too small: need %zu bytes",
                  w.total);
   B200FA_REQUIRE(reinterpret_cast<uintptr_t>(a.workspace) % 256 == 0, "backward workspace must be 256-byte aligned");
@@ -997,6 +1097,7 @@ static int launch_bwd_d(const b200fa_bwd_args& a, int sink, cudaStream_t stream)
                a.dk_stride[2] % 16 == 0 && a.dv_stride[1] % 16 == 0 && a.dv_stride[2] % 16 == 0 && bp.head_dim % 16 == 0;
   p.work_list = nullptr;
   p.n_blocks = p.head_slots = p.section = 1;
+  p.sinks = SinkShares{w.sink_rows, w.sink_blocks, 0, 0, nullptr, reinterpret_cast<float*>(ws + w.sink_part)};
   p.status = device_status_word();
   if (!p.status) return B200FA_ERR_CUDA;
   p.trace = trace_buffer();
@@ -1014,9 +1115,23 @@ static int launch_bwd_d(const b200fa_bwd_args& a, int sink, cudaStream_t stream)
                                   reinterpret_cast<int32_t*>(ws + w.work_list), stream);
     if (status != B200FA_OK) return status;
     p.work_list = reinterpret_cast<const int2*>(ws + w.work_list);
-    grid = dim3((unsigned)w.entries, (unsigned)bp.heads_kv * kHeadSplit, 1);
+    if (p.sinks.rows) {
+      status = b200fa_work_list(bp.cu_seqlens_q, bp.cu_seqlens_q, bp.batch, p.sinks.rows, 0, (int32_t)w.sink_entries,
+                                reinterpret_cast<int32_t*>(ws + w.sink_list), stream);
+      if (status != B200FA_OK) return status;
+      p.sinks.list = reinterpret_cast<const int2*>(ws + w.sink_list);
+      p.sinks.ctas = (int)w.sink_entries * p.sinks.blocks;
+    }
+    grid = dim3((unsigned)w.entries + (unsigned)p.sinks.ctas, (unsigned)bp.heads_kv * kHeadSplit, 1);
   } else if (run_main) {
-    p.n_blocks = ceil_div(bp.seqlen_k, kBlockN);
+    if (p.sinks.rows) {
+      p.sinks.blocks = imin(p.sinks.blocks, ceil_div(bp.seqlen_k, kBlockN));
+      p.sinks.per_sequence = ceil_div(bp.seqlen_q, p.sinks.rows);
+      B200FA_REQUIRE((int64_t)p.sinks.per_sequence * bp.batch * bp.heads_kv * p.sinks.blocks < INT_MAX, "too many key blocks for one backward launch");
+      p.sinks.ctas = p.sinks.per_sequence * bp.batch * bp.heads_kv * p.sinks.blocks;
+    }
+    const int dealt_out = p.sinks.rows ? p.sinks.blocks : 0;  // key blocks in front of those of the launch's main part
+    p.n_blocks = ceil_div(bp.seqlen_k, kBlockN) - dealt_out;
     p.head_slots = bp.heads_kv * kHeadSplit;
     const int64_t groups = (int64_t)p.head_slots * bp.batch;
     // Interleaving sections pays when the key blocks differ in weight (causal: the first block sees every query
@@ -1027,7 +1142,7 @@ static int launch_bwd_d(const b200fa_bwd_args& a, int sink, cudaStream_t stream)
     int64_t total_weight = 0, heaviest = 0;
     for (int nb = 0; nb < p.n_blocks; ++nb) {
       int first = 0, last = 0;
-      const int c0 = nb * kBlockN, c1 = c0 + kBlockN < bp.seqlen_k ? c0 + kBlockN : bp.seqlen_k;
+      const int c0 = (nb + dealt_out) * kBlockN, c1 = c0 + kBlockN < bp.seqlen_k ? c0 + kBlockN : bp.seqlen_k;
       sink_query_block_range(band, bp.seqlen_q, c0, c1, sink, &first, &last);
       const int64_t weight = last > first ? last - first : 0;
       total_weight += weight;
@@ -1040,8 +1155,8 @@ static int launch_bwd_d(const b200fa_bwd_args& a, int sink, cudaStream_t stream)
     const int64_t wide = p.n_blocks <= 8 ? 16 : p.n_blocks <= 16 ? 8 : kBwdSection;
     const int64_t wanted = uneven ? wide : 1;
     p.section = (int)(groups < wanted ? groups : wanted);
-    B200FA_REQUIRE(groups * p.n_blocks < INT_MAX, "too many key blocks for one backward launch");
-    grid = dim3((unsigned)(groups * p.n_blocks), 1, 1);
+    B200FA_REQUIRE(groups * p.n_blocks + p.sinks.ctas < INT_MAX, "too many key blocks for one backward launch");
+    grid = dim3((unsigned)(groups * p.n_blocks) + (unsigned)p.sinks.ctas, 1, 1);
   }
   mark(1, stream);
   if (run_main) {
@@ -1052,6 +1167,13 @@ static int launch_bwd_d(const b200fa_bwd_args& a, int sink, cudaStream_t stream)
       status = launch_main<D>(a, p, grid, dq_accum, w.rows, stream);
     }
     if (status != B200FA_OK) return status;
+    if constexpr (D <= 128) {
+      if (p.sinks.rows) {
+        const dim3 join((unsigned)(bp.batch * p.sinks.blocks * (kBlockN * D / 4 / 256)), (unsigned)bp.heads_kv);
+        bwd_sink_join_kernel<D><<<join, 256, 0, stream>>>(p);
+        B200FA_CUDA_CHECK(cudaGetLastError());
+      }
+    }
   }
   mark(2, stream);
 

@@ -17,6 +17,19 @@ constexpr float kPivotSumScale = 128.f;
 // 2^-166 stays normal, sums up to 2^87 stay finite.
 constexpr float kDkFixScale = 1099511627776.f;
 
+// Sinks make the first key blocks of a sequence heavy: every query row sees them, while the others are seen by a window of
+// rows. Their work is therefore dealt out in shares of `rows` query rows, one CTA each (rows = 0: it is not), which start
+// first and leave FP32 parts of dK and dV, added up in order by bwd_sink_join_kernel. Share i of a sequence that starts at
+// query row q0 has the slot q0 / rows + sequence + i: no two shares have the same, and there are rows_total / rows + batch.
+struct SinkShares {
+  int rows;             // query rows per share, a multiple of 128
+  int blocks;           // key blocks per sequence that hold sinks, at most
+  int ctas;             // leading CTAs (grid.x) that hold shares: fixed length over all key heads, packed per key head
+  int per_sequence;     // fixed length: shares per sequence
+  const int2* list;     // packed: (sequence, share) entries
+  float* part;          // (slots, heads_kv, blocks, dV and dK, 128, compiled width)
+};
+
 struct BwdParams {
   Problem prob;
   float scale, scale_log2;
@@ -37,6 +50,7 @@ struct BwdParams {
   int64_t dv_batch_stride, dv_row_stride, dv_head_stride;
   const int2* work_list;  // packed problems: (key sequence, key block) per blockIdx.x
   int n_blocks, head_slots, section;  // fixed length: decoding of the linear CTA index, see bwd_cta_of
+  SinkShares sinks;                   // kSink instances
   int* status;
   long long* trace;  // optional cycle counters, null = off
 };
