@@ -22,17 +22,15 @@ work_list_kernel(const int32_t* __restrict__ cu, const int32_t* __restrict__ cu_
   __shared__ uint32_t keys[kListThreads];
   __shared__ int order[kListThreads];
   __shared__ int count[kListThreads];
-  __shared__ int scan[kListThreads];
-  __shared__ int written_shared;
-  const int tid = threadIdx.x;
-  if (tid == 0) written_shared = 0;
-  __syncthreads();
+  __shared__ int warp_sums[kListThreads / 32];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  int written = 0;
   for (int first = 0; first < batch; first += kListThreads) {
     const int i = first + tid;
-    const bool valid = i < batch;
-    uint32_t key = 2 * kClasses;  // invalid entries sort last
+    const int present = imin(batch - first, kListThreads);  // sequences of this window
+    uint32_t key = 0;
     int blocks = 0;
-    if (valid) {
+    if (tid < present) {
       const uint32_t other = static_cast<uint32_t>(cu_other[i + 1] - cu_other[i]);
       key = kClasses - 1 - length_class(other);
       // A prefix-sum array that is not non-decreasing describes no batch; its negative lengths count as empty
@@ -41,38 +39,40 @@ work_list_kernel(const int32_t* __restrict__ cu, const int32_t* __restrict__ cu_
     }
     keys[tid] = key;
     __syncthreads();
-    int rank = 0;
-    for (int j = 0; j < kListThreads; ++j) {
-      const uint32_t other_key = keys[j];
-      rank += (other_key < key || (other_key == key && j < tid)) ? 1 : 0;
+    int rank = tid;  // places behind the last sequence stay where they are
+    if (tid < present) {
+      rank = 0;
+      for (int j = 0; j < present; ++j) {
+        const uint32_t other_key = keys[j];
+        rank += (other_key < key || (other_key == key && j < tid)) ? 1 : 0;
+      }
     }
     order[rank] = i;
     count[rank] = blocks;
     __syncthreads();
-    // inclusive scan of count[] (Hillis-Steele, double buffered through `scan`)
-    int value = count[tid];
-    scan[tid] = value;
-    __syncthreads();
-    for (int distance = 1; distance < kListThreads; distance <<= 1) {
-      const int add = tid >= distance ? scan[tid - distance] : 0;
-      __syncthreads();
-      value += add;
-      scan[tid] = value;
-      __syncthreads();
-    }
-    const int base = written_shared;
+    // inclusive prefix sum of count[]: within the warps, then over them
     const int my_blocks = count[tid];
-    const int start = base + value - my_blocks;
+    int value = my_blocks;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int add = __shfl_up_sync(0xffffffffu, value, d);
+      if (lane >= d) value += add;
+    }
+    if (lane == 31) warp_sums[warp] = value;
+    __syncthreads();
+    const int own = warp_sums[lane];
+    value += __reduce_add_sync(0xffffffffu, lane < warp ? own : 0);
+    const int total = __reduce_add_sync(0xffffffffu, own);
+    const int start = written + value - my_blocks;
     const int sequence = order[tid];
     for (int b = 0; b < my_blocks; ++b) {
       const int entry = start + b;
       if (entry >= 0 && entry < num_entries) table[entry] = make_int2(sequence, descending ? my_blocks - 1 - b : b);
     }
-    __syncthreads();
-    if (tid == kListThreads - 1) written_shared = base + value;
-    __syncthreads();
+    written += total;
+    __syncthreads();  // the shared arrays may be overwritten
   }
-  for (int entry = written_shared + tid; entry < num_entries; entry += kListThreads) table[entry] = make_int2(batch, 0);
+  for (int entry = written + tid; entry < num_entries; entry += kListThreads) table[entry] = make_int2(batch, 0);
 }
 
 // ------------------------------------------------------------------------------------------------ metadata
