@@ -399,11 +399,23 @@ fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CU
           __syncwarp();
         }
         auto apply_mask = [&](float2* values, int first_column) {
+          if constexpr (kSink) {
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+              const uint32_t bits = visible_columns(first_column + 32 * w, lo, hi, sinks);
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                values[16 * w + i].x = (bits & (1u << (2 * i))) ? values[16 * w + i].x : -INFINITY;
+                values[16 * w + i].y = (bits & (2u << (2 * i))) ? values[16 * w + i].y : -INFINITY;
+              }
+            }
+            return;
+          }
 #pragma unroll
           for (int i = 0; i < 32; ++i) {
             const int c = first_column + 2 * i;
-            values[i].x = column_visible<kSink>(c, lo, hi, sinks) ? values[i].x : -INFINITY;
-            values[i].y = column_visible<kSink>(c + 1, lo, hi, sinks) ? values[i].y : -INFINITY;
+            values[i].x = (c >= lo && c < hi) ? values[i].x : -INFINITY;
+            values[i].y = (c + 1 >= lo && c + 1 < hi) ? values[i].y : -INFINITY;
           }
         };
         auto max_of = [&](const float2* values) {
