@@ -382,6 +382,14 @@ bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CU
         }
         if (!key_valid) qhi = 0;
         const bool masked = __any_sync(0xffffffffu, qlo > cb || qhi < cb + C);
+        // kSink: the visible ones of this thread's query columns as bits, 32 to a word; a test of a fixed bit costs half of
+        // the two compares.
+        uint32_t seen[C / 32];
+        if constexpr (kSink) {
+#pragma unroll
+          for (int h = 0; h < C / 32; ++h)
+            seen[h] = columns_below(qhi - cb - 32 * h) & ~columns_below(qlo - cb - 32 * h);
+        }
         // ---- P^T (kept in FP32 registers for dS, stored to TMEM as BF16 for the dV MMA)
         if (!mbar_wait_traced(bar_s_full, it & 1, wctx, kWaitBwdCompute, 7, true)) { ok = false; break; }
         tc_fence_after();
@@ -416,10 +424,13 @@ bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CU
           float p0 = ex2_approx(x01.x), p1 = ex2_approx(x01.y), p2 = ex2_approx(x23.x), p3 = ex2_approx(x23.y);
           if (masked) {
             const int q = cb + 4 * j;
-            p0 = (q + 0 >= qlo && q + 0 < qhi) ? p0 : 0.f;
-            p1 = (q + 1 >= qlo && q + 1 < qhi) ? p1 : 0.f;
-            p2 = (q + 2 >= qlo && q + 2 < qhi) ? p2 : 0.f;
-            p3 = (q + 3 >= qlo && q + 3 < qhi) ? p3 : 0.f;
+            auto visible = [&](int i) {
+              return kSink ? (seen[j / 8] & (1u << (4 * (j % 8) + i))) != 0 : q + i >= qlo && q + i < qhi;
+            };
+            p0 = visible(0) ? p0 : 0.f;
+            p1 = visible(1) ? p1 : 0.f;
+            p2 = visible(2) ? p2 : 0.f;
+            p3 = visible(3) ? p3 : 0.f;
           }
           pf[4 * j + 0] = p0;
           pf[4 * j + 1] = p1;
@@ -489,10 +500,13 @@ bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CU
               float s0 = s01.x, s1 = s01.y, s2 = s23.x, s3 = s23.y;
               if (masked) {
                 const int q = cb + 32 * h + i;
-                s0 = (q + 0 >= qlo && q + 0 < qhi) ? s0 : 0.f;
-                s1 = (q + 1 >= qlo && q + 1 < qhi) ? s1 : 0.f;
-                s2 = (q + 2 >= qlo && q + 2 < qhi) ? s2 : 0.f;
-                s3 = (q + 3 >= qlo && q + 3 < qhi) ? s3 : 0.f;
+                auto visible = [&](int e2) {
+                  return kSink ? (seen[h] & (1u << (i + e2))) != 0 : q + e2 >= qlo && q + e2 < qhi;
+                };
+                s0 = visible(0) ? s0 : 0.f;
+                s1 = visible(1) ? s1 : 0.f;
+                s2 = visible(2) ? s2 : 0.f;
+                s3 = visible(3) ? s3 : 0.f;
               }
               packed[2 * e] = pack_bf16x2(s0, s1);
               packed[2 * e + 1] = pack_bf16x2(s2, s3);
@@ -942,6 +956,20 @@ static int sink_share_rows(const b200fa_problem& p, int sink) {
   const int64_t average = p.heads_kv * row_blocks * (window_blocks + ceil_div(sink, kBlockN)) / 148;
   int64_t blocks = window_blocks > 4 ? window_blocks : 4;
   if (blocks < average / 8) blocks = average / 8;
+  if (!packed) {
+    // One CTA runs per SM, so a launch of two or three waves ends with a full or an almost empty one depending on the number
+    // of shares: take the size, up to twice the smallest, with the least product of waves and largest CTA (2 x 4096 tokens,
+    // 16/4 heads, window 512: six blocks, two waves instead of five blocks, three waves).
+    const int64_t pairs = (int64_t)p.batch * p.heads_kv, sink_blocks = ceil_div(sink, kBlockN);
+    const int64_t others = pairs * (ceil_div(p.seqlen_k, kBlockN) - sink_blocks), rows = ceil_div(p.seqlen_q, kBlockM);
+    int64_t best = 0, best_cost = 0;
+    for (int64_t size = blocks; size <= 2 * blocks; ++size) {
+      const int64_t ctas = others + pairs * sink_blocks * ((rows + size - 1) / size);
+      const int64_t cost = (ctas + 147) / 148 * (size > window_blocks ? size : window_blocks);
+      if (best == 0 || cost < best_cost) best = size, best_cost = cost;
+    }
+    blocks = best;
+  }
   if (blocks * 2 * kBlockM > (int64_t)p.seqlen_q) return 0;  // (packed: no sequence can have two shares)
   return (int)(blocks * kBlockM);
 }

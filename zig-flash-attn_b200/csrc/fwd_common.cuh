@@ -74,12 +74,6 @@ __device__ __forceinline__ bool column_visible(int c, int lo, int hi, int sinks)
   return (c >= lo || (kSink && c < sinks)) && c < hi;
 }
 
-// Bits of the columns below `x` of a word of 32 columns (x may lie on either side of the word).
-__device__ __forceinline__ uint32_t columns_below(int x) {
-  uint32_t bits;
-  asm("bmsk.clamp.b32 %0, 0, %1;" : "=r"(bits) : "r"(imax(x, 0)));
-  return bits;
-}
 // The visible ones of 32 columns that start at column `first` of the block, as bits (kSink instances: two intervals). A
 // bit test with a fixed position costs less than half of the three compares per score that the limits would take.
 __device__ __forceinline__ uint32_t visible_columns(int first, int lo, int hi, int sinks) {

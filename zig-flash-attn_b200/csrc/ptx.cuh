@@ -394,6 +394,12 @@ __device__ __forceinline__ float2 ex2_poly2(float2 x) {
   result.y = x.y > -127.f ? result.y : 0.f;
   return result;
 }
+// Bits of the columns below `x` of a word of 32 columns (x may lie on either side of the word).
+__device__ __forceinline__ uint32_t columns_below(int x) {
+  uint32_t bits;
+  asm("bmsk.clamp.b32 %0, 0, %1;" : "=r"(bits) : "r"(x > 0 ? x : 0));
+  return bits;
+}
 // 32-byte store to global memory (the address must be 32-byte aligned).
 __device__ __forceinline__ void st_global_v8(void* address, const uint32_t* w) {
   asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(address), "r"(w[0]), "r"(w[1]), "r"(w[2]),
