@@ -8,6 +8,7 @@
 #include <cooperative_groups.h>
 
 #include "common.h"
+#include "fwd_common.cuh"
 #include "ptx.cuh"
 
 namespace b200fa {
@@ -19,7 +20,8 @@ struct CacheView {
   uint8_t* k;
   uint8_t* v;
   int64_t k_page, k_row, k_head, v_page, v_row, v_head;  // strides in bytes
-  int num_pages, page_size, heads, chunks;               // chunks = 16-byte pieces of a row
+  int num_pages, page_size, heads;
+  FastDiv chunks, row_chunks;  // 16-byte pieces of a row of a head, and of all heads
 };
 
 struct AppendParams {
@@ -34,7 +36,9 @@ struct AppendParams {
   int batch, capacity;
 };
 
-// One warp per token: finds its sequence (binary search in the prefix sums of a packed batch), its page and its row.
+// One warp per token: finds its sequence (binary search in the prefix sums of a packed batch), its page and its row, then
+// copies the heads' pieces, four of each tensor in flight. HBM-bound from a few thousand tokens on: 31 k tokens of 8 x 128
+// (129 MB moved) in 23 us; below that the chain length -> table -> page of dependent loads is what it takes, 4 us.
 __global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ AppendParams p) {
   const int64_t token = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
@@ -52,36 +56,68 @@ __global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ App
     index = token - p.cu_seqlens[b];
   } else {
     if (token >= p.rows * p.batch) return;
-    b = (int)(token / p.rows);
-    row = index = token - b * p.rows;
+    b = (int)token / (int)p.rows;  // both below 2^31
+    row = index = token - (int64_t)b * p.rows;
   }
   const int64_t position = p.lengths[b] + index;
   if (position < 0 || position >= p.capacity) return;
-  const int page = p.table[b * p.table_seq + position / p.cache.page_size];
+  const int entry = (int)position / p.cache.page_size, slot = (int)position - entry * p.cache.page_size;
+  const int page = p.table[b * p.table_seq + entry];
   if (page < 0 || page >= p.cache.num_pages) return;
-  const int64_t slot = position % p.cache.page_size;
   const int64_t seq = p.cu_seqlens ? 0 : b;
-  for (int i = lane; i < p.cache.heads * p.cache.chunks; i += 32) {
-    const int head = i / p.cache.chunks, chunk = i - head * p.cache.chunks;
-    *reinterpret_cast<uint4*>(p.cache.k + page * p.cache.k_page + slot * p.cache.k_row + head * p.cache.k_head + 16 * chunk) =
-        *reinterpret_cast<const uint4*>(p.k + seq * p.k_seq + row * p.k_row + head * p.k_head + 16 * chunk);
-    *reinterpret_cast<uint4*>(p.cache.v + page * p.cache.v_page + slot * p.cache.v_row + head * p.cache.v_head + 16 * chunk) =
-        *reinterpret_cast<const uint4*>(p.v + seq * p.v_seq + row * p.v_row + head * p.v_head + 16 * chunk);
+  const uint8_t* k_from = p.k + seq * p.k_seq + row * p.k_row;
+  const uint8_t* v_from = p.v + seq * p.v_seq + row * p.v_row;
+  uint8_t* k_to = p.cache.k + page * p.cache.k_page + slot * p.cache.k_row;
+  uint8_t* v_to = p.cache.v + page * p.cache.v_page + slot * p.cache.v_row;
+  const int pieces = (int)p.cache.row_chunks.divisor;
+  for (int base = lane; base < pieces; base += 128) {
+    uint4 k[4], v[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int i = base + 32 * u, head = p.cache.chunks.div(i), at = 16 * (i - head * (int)p.cache.chunks.divisor);
+      if (i < pieces) {
+        k[u] = *reinterpret_cast<const uint4*>(k_from + head * p.k_head + at);
+        v[u] = *reinterpret_cast<const uint4*>(v_from + head * p.v_head + at);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int i = base + 32 * u, head = p.cache.chunks.div(i), at = 16 * (i - head * (int)p.cache.chunks.divisor);
+      if (i < pieces) {
+        *reinterpret_cast<uint4*>(k_to + head * p.cache.k_head + at) = k[u];
+        *reinterpret_cast<uint4*>(v_to + head * p.cache.v_head + at) = v[u];
+      }
+    }
   }
 }
 
-// One block per pair of pages; pairs with an entry outside [0, num_pages) are skipped.
+// Page copies: one block per (pair, 16 KiB of a page, cache), so that a few pairs of large pages keep every SM busy as well
+// as thousands of small ones do; a thread has four 16-byte pieces in flight. Pairs with an entry outside [0, num_pages) are
+// skipped. HBM-bound: 3932 pairs of 32 KiB pages, 515 MB moved, in 83 us (6.2 TB/s); 64 pairs of 128 KiB pages in 6 us, with one
+// block per pair 36 us.
+constexpr int kCopyPieces = 1024;
 __global__ void __launch_bounds__(256) copy_pages_kernel(const __grid_constant__ CacheView c, const int32_t* source,
                                                          const int32_t* target) {
   const int from = source[blockIdx.x], to = target[blockIdx.x];
   if (from < 0 || to < 0 || from >= c.num_pages || to >= c.num_pages || from == to) return;
-  for (int i = threadIdx.x; i < c.page_size * c.heads * c.chunks; i += 256) {
-    const int row = i / (c.heads * c.chunks), rest = i - row * (c.heads * c.chunks);
-    const int head = rest / c.chunks, chunk = rest - head * c.chunks;
-    const int64_t k_at = row * c.k_row + head * c.k_head + 16 * chunk, v_at = row * c.v_row + head * c.v_head + 16 * chunk;
-    *reinterpret_cast<uint4*>(c.k + to * c.k_page + k_at) = *reinterpret_cast<const uint4*>(c.k + from * c.k_page + k_at);
-    *reinterpret_cast<uint4*>(c.v + to * c.v_page + v_at) = *reinterpret_cast<const uint4*>(c.v + from * c.v_page + v_at);
+  const bool is_v = blockIdx.z;
+  const int64_t row_stride = is_v ? c.v_row : c.k_row, head_stride = is_v ? c.v_head : c.k_head;
+  const uint8_t* read = is_v ? c.v + from * c.v_page : c.k + from * c.k_page;
+  uint8_t* write = is_v ? c.v + to * c.v_page : c.k + to * c.k_page;
+  const int pieces = c.page_size * (int)c.row_chunks.divisor, first = blockIdx.y * kCopyPieces + threadIdx.x;
+  uint4 data[kCopyPieces / 256];
+  int64_t at[kCopyPieces / 256];
+#pragma unroll
+  for (int u = 0; u < kCopyPieces / 256; ++u) {
+    const int i = first + 256 * u;
+    const int row = c.row_chunks.div(i), rest = i - row * (int)c.row_chunks.divisor;
+    const int head = c.chunks.div(rest), chunk = rest - head * (int)c.chunks.divisor;
+    at[u] = row * row_stride + head * head_stride + 16 * chunk;
+    if (i < pieces) data[u] = *reinterpret_cast<const uint4*>(read + at[u]);
   }
+#pragma unroll
+  for (int u = 0; u < kCopyPieces / 256; ++u)
+    if (first + 256 * u < pieces) *reinterpret_cast<uint4*>(write + at[u]) = data[u];
 }
 
 // ---------------------------------------------------------------------------------------------- bookkeeping
@@ -152,6 +188,23 @@ __device__ __forceinline__ int team_scan(cg::cluster_group team, int value, int*
   return total;
 }
 
+// visit(row, entry, load(row, entry)) for all entries of the rows [begin, end), a warp per row, four loads of a lane in flight
+// (sixteen measured the same).
+template <typename Load, typename Visit>
+__device__ __forceinline__ void for_rows(int begin, int end, int columns, Load load, Visit visit) {
+  const int lane = threadIdx.x & 31;
+  for (int row = begin + (threadIdx.x >> 5); row < end; row += kTeamThreads / 32) {
+    for (int base = lane; base < columns; base += 128) {
+      int value[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) value[u] = base + 32 * u < columns ? load(row, base + 32 * u) : -1;
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (base + 32 * u < columns) visit(row, base + 32 * u, value[u]);
+    }
+  }
+}
+
 struct Range {
   int begin, end;
 };
@@ -160,23 +213,30 @@ __device__ __forceinline__ Range team_range(cg::cluster_group team, int count) {
   return {begin, imin(begin + each, count)};
 }
 
-// scratch[r] = r-th free page for r < wanted, refs_out[page] = 1 for these (where mark is set) and refs otherwise.
-__device__ __forceinline__ void list_free_pages(const PagesParams& p, Range pages, int free_before, int wanted,
-                                                int* warp_sums, bool mark) {
-  int rank = free_before;
+// Walks a range of pages in order: visit(page, count, is, before) with the page's reference count, whether test(count) holds,
+// and for how many pages in front of it test holds, `before` the range included. (Eight pages per thread and round: the
+// same or slower.)
+template <typename Test, typename Visit>
+__device__ __forceinline__ void rank_pages(const PagesParams& p, Range pages, int before, int* warp_sums, Test test, Visit visit) {
   for (int base = pages.begin; base < pages.end; base += kTeamThreads) {
     const int page = base + threadIdx.x;
-    const int count = page < pages.end ? p.refs[page] : 1;
-    const bool is_free = count <= 0;
+    const int count = page < pages.end ? p.refs[page] : 0;
+    const bool is = page < pages.end && test(count);
     int total;
-    const int at = rank + block_scan(is_free, warp_sums, &total);
-    if (page < pages.end) {
-      const bool taken = is_free && at < wanted;
-      if (taken) p.scratch[at] = page;
-      p.refs_out[page] = taken && mark ? 1 : count;
-    }
-    rank += total;
+    const int rank = before + block_scan(is, warp_sums, &total);
+    if (page < pages.end) visit(page, count, is, rank);
+    before += total;
   }
+}
+
+// scratch[r] = r-th free page and refs_out[page] = 1 for r < wanted; the other counts are copied.
+__device__ __forceinline__ void list_free_pages(const PagesParams& p, Range pages, int free_before, int wanted, int* warp_sums) {
+  rank_pages(p, pages, free_before, warp_sums, [](int count) { return count <= 0; },
+             [&](int page, int count, bool is_free, int rank) {
+               const bool taken = is_free && rank < wanted;
+               if (taken) p.scratch[rank] = page;
+               p.refs_out[page] = taken ? 1 : count;
+             });
 }
 
 __device__ __forceinline__ int count_free(const PagesParams& p, Range pages, int* warp_sums) {
@@ -209,12 +269,9 @@ reserve_pages_kernel(const __grid_constant__ PagesParams p) {
   int requests_before, free_before;
   const int requests = team_scan(team, requests_here, &exchange[0], &requests_before);
   const int free_pages = team_scan(team, free_here, &exchange[1], &free_before);
-  list_free_pages(p, pages, free_before, requests, warp_sums, true);
-  for (int64_t i = (int64_t)seqs.begin * p.max_pages + threadIdx.x; i < (int64_t)seqs.end * p.max_pages; i += kTeamThreads) {
-    const int b = (int)(i / p.max_pages), entry = (int)(i - (int64_t)b * p.max_pages);
-    const int page = p.table[b * p.table_seq + entry];
-    p.table_out[i] = holds_page(p, page) ? page : -1;
-  }
+  list_free_pages(p, pages, free_before, requests, warp_sums);
+  for_rows(seqs.begin, seqs.end, p.max_pages, [&](int b, int entry) { return p.table[b * p.table_seq + entry]; },
+           [&](int b, int entry, int page) { p.table_out[(int64_t)b * p.max_pages + entry] = holds_page(p, page) ? page : -1; });
   team.sync();  // the list of free pages and the copies of the rows are complete
   int rank = requests_before;
   for (int base = seqs.begin; base < seqs.end; base += kTeamThreads) {
@@ -266,7 +323,7 @@ fork_pages_kernel(const __grid_constant__ PagesParams p) {
   int requests_before, free_before;
   const int requests = team_scan(team, requests_here, &exchange[0], &requests_before);
   const int free_pages = team_scan(team, free_here, &exchange[1], &free_before);
-  list_free_pages(p, pages, free_before, requests, warp_sums, true);
+  list_free_pages(p, pages, free_before, requests, warp_sums);
   team.sync();  // the list of free pages and the copy of the counts are complete
   int rank = requests_before;
   for (int base = children.begin; base < children.end; base += kTeamThreads) {
@@ -285,37 +342,38 @@ fork_pages_kernel(const __grid_constant__ PagesParams p) {
     rank += total;
   }
   __syncthreads();  // the targets of this block's children
-  for (int64_t i = (int64_t)children.begin * p.max_pages + threadIdx.x; i < (int64_t)children.end * p.max_pages;
-       i += kTeamThreads) {
-    const int child = (int)(i / p.max_pages), entry = (int)(i - (int64_t)child * p.max_pages);
-    const int full = p.lengths_out[child] / p.page_size;
-    int page = -1;
-    if (entry < full) {
-      page = p.table[p.extra[child] * p.table_seq + entry];
-      if (holds_page(p, page)) atomicAdd(&p.refs_out[page], 1); else page = -1;
-    } else if (entry == full) {
-      page = p.target[child];
-    }
-    p.table_out[i] = page;
-  }
+  for_rows(
+      children.begin, children.end, p.max_pages,
+      [&](int child, int entry) {
+        const int full = p.lengths_out[child] / p.page_size;
+        return entry < full ? p.table[p.extra[child] * p.table_seq + entry] : entry == full ? p.target[child] : -1;
+      },
+      [&](int child, int entry, int page) {
+        if (!holds_page(p, page)) page = -1;
+        else if (entry < p.lengths_out[child] / p.page_size) atomicAdd(&p.refs_out[page], 1);
+        p.table_out[(int64_t)child * p.max_pages + entry] = page;
+      });
 }
 
-__global__ void __cluster_dims__(kTeamBlocks) __launch_bounds__(kTeamThreads)
-free_pages_kernel(const __grid_constant__ PagesParams p) {
-  const cg::cluster_group team = cg::this_cluster();
-  const Range seqs = team_range(team, p.sequences), pages = team_range(team, p.num_pages);
-  for (int page = pages.begin + threadIdx.x; page < pages.end; page += kTeamThreads) p.refs_out[page] = p.refs[page];
-  team.sync();
-  for (int64_t i = (int64_t)seqs.begin * p.max_pages + threadIdx.x; i < (int64_t)seqs.end * p.max_pages; i += kTeamThreads) {
-    const int b = (int)(i / p.max_pages), entry = (int)(i - (int64_t)b * p.max_pages);
-    int page = p.table[b * p.table_seq + entry];
+// refs_out holds a copy of the counts. No order between the rows is needed, so this one runs on the whole GPU, a warp per
+// row: 512 rows of 502 entries, 95 k of them freed, with the copy in 7 us, as one cluster 15 us (8 SMs are slow at the
+// reductions).
+__global__ void __launch_bounds__(256) free_pages_kernel(const __grid_constant__ PagesParams p) {
+  const int lane = threadIdx.x & 31, b = blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (b >= p.sequences) return;
+  const int first = p.extra[b], last = p.extra2[b];
+  const int32_t* row = p.table + b * p.table_seq;
+  int32_t* row_out = p.table_out + (int64_t)b * p.max_pages;
+#pragma unroll 4
+  for (int entry = lane; entry < p.max_pages; entry += 32) {
+    int page = row[entry];
     if (!holds_page(p, page)) {
       page = -1;
-    } else if (entry >= p.extra[b] && entry < p.extra2[b]) {
+    } else if (entry >= first && entry < last) {
       atomicSub(&p.refs_out[page], 1);
       page = -1;
     }
-    p.table_out[i] = page;
+    row_out[entry] = page;
   }
 }
 
@@ -330,19 +388,12 @@ compact_pages_kernel(const __grid_constant__ PagesParams p) {
   for (int page = pages.begin + threadIdx.x; page < imin(pages.end, live); page += kTeamThreads) mine += p.refs[page] > 0;
   const int kept = team_scan(team, block_sum(mine, warp_sums), &exchange[1], &kept_before);
   const int moves = live - kept;
-  int rank = live_before;
-  for (int base = pages.begin; base < pages.end; base += kTeamThreads) {
-    const int page = base + threadIdx.x;
-    const bool is_live = page < pages.end && p.refs[page] > 0;
-    int total;
-    const int at = rank + block_scan(is_live, warp_sums, &total);
-    if (page < pages.end) {
-      if (is_live && page >= live) p.source[at - kept] = page;
-      if (!is_live && page < live) p.target[page - at] = page;
-      p.refs_out[page] = page < live ? p.refs[page] : 0;
-    }
-    rank += total;
-  }
+  rank_pages(p, pages, live_before, warp_sums, [](int count) { return count > 0; },
+             [&](int page, int count, bool is_live, int rank) {
+               if (is_live && page >= live) p.source[rank - kept] = page;
+               if (!is_live && page < live) p.target[page - rank] = page;
+               p.refs_out[page] = page < live ? count : 0;
+             });
   team.sync();
   for (int i = (int)team.block_rank() * kTeamThreads + threadIdx.x; i < p.pairs; i += kTeamBlocks * kTeamThreads) {
     if (i < moves) {
@@ -355,13 +406,13 @@ compact_pages_kernel(const __grid_constant__ PagesParams p) {
     }
   }
   team.sync();
-  for (int64_t i = (int64_t)seqs.begin * p.max_pages + threadIdx.x; i < (int64_t)seqs.end * p.max_pages; i += kTeamThreads) {
-    const int b = (int)(i / p.max_pages), entry = (int)(i - (int64_t)b * p.max_pages);
-    int page = p.table[b * p.table_seq + entry];
-    if (!holds_page(p, page) || p.refs[page] <= 0) page = -1;
-    else if (page >= live) page = p.scratch[page];
-    p.table_out[i] = page;
-  }
+  for_rows(seqs.begin, seqs.end, p.max_pages,
+           [&](int b, int entry) {
+             const int page = p.table[b * p.table_seq + entry];
+             if (!holds_page(p, page) || p.refs[page] <= 0) return -1;
+             return page >= live ? p.scratch[page] : page;
+           },
+           [&](int b, int entry, int page) { p.table_out[(int64_t)b * p.max_pages + entry] = page; });
 }
 
 // ---------------------------------------------------------------------------------------------- host side
@@ -379,7 +430,8 @@ static int cache_view(const b200fa_kv_cache& c, CacheView* view) {
   view->v = static_cast<uint8_t*>(c.v_cache);
   view->k_page = 2 * c.k_stride[0], view->k_row = 2 * c.k_stride[1], view->k_head = 2 * c.k_stride[2];
   view->v_page = 2 * c.v_stride[0], view->v_row = 2 * c.v_stride[1], view->v_head = 2 * c.v_stride[2];
-  view->num_pages = c.num_pages, view->page_size = c.page_size, view->heads = c.heads_kv, view->chunks = c.head_dim / 8;
+  view->num_pages = c.num_pages, view->page_size = c.page_size, view->heads = c.heads_kv;
+  view->chunks = FastDiv::make((uint32_t)c.head_dim / 8), view->row_chunks = FastDiv::make((uint32_t)(c.heads_kv * (c.head_dim / 8)));
   return B200FA_OK;
 }
 
@@ -450,7 +502,10 @@ int b200fa_copy_pages(const b200fa_kv_cache* cache, const int32_t* source_pages,
   B200FA_REQUIRE(count >= 0, "negative sizes");
   if (count == 0 || cache->num_pages == 0) return B200FA_OK;
   B200FA_REQUIRE(source_pages && target_pages, "null tensor pointer");
-  copy_pages_kernel<<<(unsigned)count, 256, 0, static_cast<cudaStream_t>(stream)>>>(view, source_pages, target_pages);
+  const int64_t pieces = (int64_t)cache->page_size * cache->heads_kv * (cache->head_dim / 8);
+  const int64_t parts = (pieces + kCopyPieces - 1) / kCopyPieces;
+  B200FA_REQUIRE(parts < 65536, "a page is larger than 1 GiB");
+  copy_pages_kernel<<<dim3((unsigned)count, (unsigned)parts, 2), 256, 0, static_cast<cudaStream_t>(stream)>>>(view, source_pages, target_pages);
   B200FA_CUDA_CHECK(cudaGetLastError());
   return B200FA_OK;
 }
@@ -492,7 +547,11 @@ int b200fa_free_pages(const b200fa_pages_args* a, const int32_t* first_entry, co
   B200FA_REQUIRE(a->sequences == 0 || (first_entry && last_entry), "null tensor pointer");
   p.extra = first_entry;
   p.extra2 = last_entry;
-  free_pages_kernel<<<kTeamBlocks, kTeamThreads, 0, static_cast<cudaStream_t>(stream)>>>(p);
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (a->num_pages > 0)
+    B200FA_CUDA_CHECK(cudaMemcpyAsync(a->page_refs_out, a->page_refs, (size_t)a->num_pages * 4, cudaMemcpyDeviceToDevice, s));
+  if (a->sequences == 0 || a->max_pages == 0) return B200FA_OK;
+  free_pages_kernel<<<(unsigned)((a->sequences + 7) / 8), 256, 0, s>>>(p);
   B200FA_CUDA_CHECK(cudaGetLastError());
   return B200FA_OK;
 }
