@@ -181,39 +181,52 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     fence_barrier_init();
   }
 
-  // ---- this block's range: steps [position, last) of the pairs in the order (chunk, sequence, step)
-  int64_t round = 0, before = 0;  // steps of all sequences; of those in front of this thread's
-  int mine = 0;
-  for (int base = 0; base < p.batch; base += kThreads) {
-    const int b = base + threadIdx.x;
-    mine = b < p.batch ? steps_of(p, b) : 0;
-    before = prefix_sum<kThreads>(mine, &round, warp_sums);
-  }
-  const Deal deal(round * p.columns, p.ranges);
-  if (blockIdx.x >= deal.ranges) {
-    if (threadIdx.x == 0) p.cut[blockIdx.x] = make_int4(-1, 0, 0, 0);
-    return;
-  }
-  int64_t position = deal.start(blockIdx.x);
-  const int64_t last = deal.start(blockIdx.x + 1);
-  int chunk = (int)quotient(position, round);
-  {
+  // ---- this block's range: steps [position, last) of the pairs in the order (chunk, sequence, step), or, where the table is
+  // too short for pairs to be cut, pairs [position, last)
+  const bool whole_pairs = p.cut == nullptr;
+  int64_t position, last, pair_start;
+  int chunk, b;
+  Deal deal(1, 1);
+  if (whole_pairs) {
+    const int64_t pairs = (int64_t)p.columns * p.batch;
+    position = quotient(pairs * blockIdx.x, gridDim.x);
+    last = quotient(pairs * (blockIdx.x + 1), gridDim.x);
+    pair_start = position;
+    chunk = (int)quotient(position, p.batch);
+    b = (int)(position - (int64_t)chunk * p.batch);
+    __syncthreads();  // the barriers are initialised
+  } else {
+    int64_t round = 0, before = 0;  // steps of all sequences; of those in front of this thread's
+    int mine = 0;
+    for (int base = 0; base < p.batch; base += kThreads) {
+      const int seq = base + threadIdx.x;
+      mine = seq < p.batch ? steps_of(p, seq) : 0;
+      before = prefix_sum<kThreads>(mine, &round, warp_sums);
+    }
+    deal = Deal(round * p.columns, p.ranges);
+    if (blockIdx.x >= deal.ranges) {
+      if (threadIdx.x == 0) p.cut[blockIdx.x] = make_int4(-1, 0, 0, 0);
+      return;
+    }
+    position = deal.start(blockIdx.x);
+    last = deal.start(blockIdx.x + 1);
+    chunk = (int)quotient(position, round);
     const int64_t offset = position - chunk * round;
     if (p.batch <= kThreads) {
       if (before <= offset && offset < before + mine) found = threadIdx.x, found_first = before;
     } else {
       int64_t total = 0;
       for (int base = 0; base < p.batch && total <= offset; base += kThreads) {
-        const int b = base + threadIdx.x;
-        mine = b < p.batch ? steps_of(p, b) : 0;
+        const int seq = base + threadIdx.x;
+        mine = seq < p.batch ? steps_of(p, seq) : 0;
         before = prefix_sum<kThreads>(mine, &total, warp_sums);
-        if (before <= offset && offset < before + mine) found = b, found_first = before;
+        if (before <= offset && offset < before + mine) found = seq, found_first = before;
       }
     }
+    __syncthreads();
+    b = found;
+    pair_start = chunk * round + found_first;
   }
-  __syncthreads();
-  int b = found;
-  int64_t pair_start = chunk * round + found_first;
 
   const uint32_t ring = smem_u32(smem) + warp * kStages * Cfg::kStepBytes, bars = smem_u32(&barriers[warp][0]);
   // Where this lane finds its pieces in the ring slot of a step. TMA: panels of 16 keys x 64 columns, 128 bytes a key, the
@@ -229,9 +242,9 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     const PagedRange range = paged_range(p.lengths[b], p.capacity, p.window_left, p.sink);
     const int pair_steps = imax(1, range.steps);
     const int begin = (int)(position - pair_start);
-    const int end = last - pair_start < pair_steps ? (int)(last - pair_start) : pair_steps;
+    const int end = whole_pairs || last - pair_start >= pair_steps ? pair_steps : (int)(last - pair_start);
     const bool whole = begin == 0 && end == pair_steps;
-    if (first_pair && threadIdx.x == 0)
+    if (first_pair && !whole_pairs && threadIdx.x == 0)
       p.cut[blockIdx.x] = begin == 0 ? make_int4(-1, 0, 0, 0)
                                      : make_int4(b, chunk, deal.owner(pair_start), deal.owner(pair_start + pair_steps - 1));
     const int32_t* table = p.table + b * p.table_seq;
@@ -482,7 +495,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     }
     if constexpr (kTma) fence_proxy_async_smem();
     __syncthreads();  // the ring is free for the copies of the next pair
-    position = pair_start = pair_start + end;
+    position = pair_start = whole_pairs ? position + 1 : pair_start + end;
     if (++b == p.batch) {
       b = 0;
       ++chunk;
@@ -555,6 +568,10 @@ struct PagedShape {
   size_t o_bytes, ml_bytes, cut_bytes;
   size_t total() const { return o_bytes + ml_bytes + cut_bytes; }
 };
+// Pairs of at most so many steps, five or six per warp of a block, are not cut: up to there the plan and the join kernel take
+// longer than the steps of one block. One sequence, 32/8 heads of 128: 256 keys 6.3 us uncut and 9.1 us cut, 512 keys 9.1
+// and 8.9, 1024 keys 13.6 and 9.4; on the host 16 us a call and 20.
+static int uncut_steps(int head_dim) { return head_dim <= 128 ? 32 : 16; }
 static PagedShape paged_shape(const b200fa_paged_args& a) {
   PagedShape s;
   const int group = a.heads_q / a.heads_kv;
@@ -564,6 +581,12 @@ static PagedShape paged_shape(const b200fa_paged_args& a) {
   const int blocks_per_sm = a.head_dim <= 256 ? 2 : 1;
   const int64_t most_work = most_steps * a.batch * a.heads_kv * s.chunks, wanted = (most_work + kMinSteps - 1) / kMinSteps;
   s.ranges = wanted < blocks_per_sm * kPagedSms ? (int)wanted : blocks_per_sm * kPagedSms;
+  s.o_bytes = s.ml_bytes = s.cut_bytes = 0;
+  if (most_steps <= uncut_steps(a.head_dim) + 1) {
+    const int64_t pairs = (int64_t)a.batch * a.heads_kv * s.chunks;
+    s.ranges = pairs < blocks_per_sm * kPagedSms ? (int)pairs : blocks_per_sm * kPagedSms;
+    return s;
+  }
   const size_t slots = 2 * (size_t)s.ranges * 8 * s.tiles;
   s.o_bytes = slots * a.head_dim * 4;
   s.ml_bytes = slots * 8;
@@ -638,7 +661,7 @@ int b200fa_paged_decode(const b200fa_paged_args* a, void* stream) {
   int status = validate_paged(a);
   if (status != B200FA_OK || a->batch == 0) return status;
   const PagedShape shape = paged_shape(*a);
-  B200FA_REQUIRE(a->workspace && a->workspace_bytes >= shape.total(), "paged attention workspace is too small: need %zu bytes",
+  B200FA_REQUIRE(shape.total() == 0 || (a->workspace && a->workspace_bytes >= shape.total()), "paged attention workspace is too small: need %zu bytes",
                  shape.total());
   B200FA_REQUIRE(reinterpret_cast<uintptr_t>(a->workspace) % 16 == 0, "paged attention workspace must be 16-byte aligned");
   PagedParams p;
@@ -654,7 +677,7 @@ int b200fa_paged_decode(const b200fa_paged_args* a, void* stream) {
   uint8_t* workspace = static_cast<uint8_t*>(a->workspace);
   p.o_part = reinterpret_cast<float*>(workspace);
   p.ml_part = reinterpret_cast<float2*>(workspace + shape.o_bytes);
-  p.cut = reinterpret_cast<int4*>(workspace + shape.o_bytes + shape.ml_bytes);
+  p.cut = shape.total() ? reinterpret_cast<int4*>(workspace + shape.o_bytes + shape.ml_bytes) : nullptr;
   p.q_seq = a->q_stride[0], p.q_head = a->q_stride[1], p.out_seq = a->out_stride[0], p.out_head = a->out_stride[1];
   p.k_page = a->k_stride[0], p.k_row = a->k_stride[1], p.k_head = a->k_stride[2];
   p.v_page = a->v_stride[0], p.v_row = a->v_stride[1], p.v_head = a->v_stride[2];
@@ -679,7 +702,7 @@ int b200fa_paged_decode(const b200fa_paged_args* a, void* stream) {
                                 : launch_paged<512>(shape.tiles, maps, p, s);
   if (status != B200FA_OK) return status;
   B200FA_CUDA_CHECK(cudaGetLastError());
-  if (shape.ranges > 1) {
+  if (p.cut && shape.ranges > 1) {
     cudaLaunchAttribute attribute;
     attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attribute.val.programmaticStreamSerializationAllowed = 1;

@@ -160,14 +160,14 @@ def _paged_forward(q, k_cache, v_cache, block_table, cache_seqlens, softmax_scal
     out = torch.empty_like(q, memory_format=torch.contiguous_format)
     softmax_lse = q.new_empty((batch, heads_q), dtype=torch.float32)
     nbytes = _paged_workspace(batch, heads_q, heads_kv, head_dim, page_size, max_pages)
-    workspace = q.new_empty((nbytes,), dtype=torch.uint8)
+    workspace = q.new_empty((nbytes,), dtype=torch.uint8) if nbytes else None
     q_stride, k_stride, v_stride = q.stride(), k_cache.stride(), v_cache.stride()
     packed = PACK_PAGED(
         batch, heads_q, heads_kv, head_dim, num_pages, page_size, max_pages, window_left, sink_size, softmax_scale,
         q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), cache_seqlens.data_ptr(), out.data_ptr(),
         softmax_lse.data_ptr(), q_stride[0], q_stride[1], k_stride[0], k_stride[1], k_stride[2],
         v_stride[0], v_stride[1], v_stride[2], heads_q * head_dim, head_dim, _table_stride(block_table),
-        workspace.data_ptr(), nbytes,
+        workspace.data_ptr() if nbytes else 0, nbytes,
     )
     on_device(device, entry("b200fa_paged_decode", ctypes.c_void_p), packed, stream_of(device))
     return out, softmax_lse
