@@ -155,10 +155,6 @@ static int validate_sinks(const b200fa_problem& p, int sink_size) {
   B200FA_REQUIRE(sink_size == 0 || !p.visibility_bits, "inter-sequence attention has no sinks");
   // masked scores are -inf before they are scaled
   B200FA_REQUIRE(sinks_of(p, sink_size) == 0 || p.softmax_scale > 0.f, "attention with sinks needs a positive softmax_scale");
-  if (sinks_of(p, sink_size) > 0 && p.head_dim > 128) {
-    set_error("attention with sinks supports head_dim 64, 72, 96 and 128, got %d", p.head_dim);
-    return B200FA_ERR_UNSUPPORTED;
-  }
   return B200FA_OK;
 }
 

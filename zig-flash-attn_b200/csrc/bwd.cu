@@ -68,13 +68,6 @@ struct BwdConfig {
   static constexpr int kTmemS = 0, kTmemDp = 128, kTmemDv = 256, kTmemDk = 256 + D;
 };
 
-// Zeroes row r of a 128-row tile of D columns (panels of 64 columns, 128 bytes a row; the swizzle stays within a row).
-template <int D>
-__device__ __forceinline__ void zero_row(uint32_t tile, int r) {
-#pragma unroll 1
-  for (int i = 0; i < D / 8; ++i) st_shared_zero16(tile + (i >> 3) * (kBlockM * 128) + r * 128 + (i & 7) * 16);
-}
-
 // kSink: window attention whose first keys stay visible (b200fa_sink_bwd), an instance of its own so that the others keep
 // their code.
 template <int D, bool kPivot, bool kSink>
@@ -86,42 +79,9 @@ bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CU
   using Cursor = QueryCursorT<!kSink, kSink>;
   const Problem& pr = p.prob;
   // ---- work item (uniform over the CTA; exits before any barrier or TMEM allocation)
-  int seq, n_block, kv_head, share = -1;
-  if (kSink && blockIdx.x < p.sinks.ctas) {
-    // a share of a key block that holds sinks
-    const int entry = blockIdx.x / p.sinks.blocks;
-    n_block = blockIdx.x - entry * p.sinks.blocks;
-    if (p.sinks.list) {
-      const int2 e = p.sinks.list[entry];
-      seq = e.x;
-      share = e.y;
-      kv_head = blockIdx.y;
-      if (seq >= pr.batch) return;
-    } else {
-      const int pair = entry / p.sinks.per_sequence;
-      share = entry - pair * p.sinks.per_sequence;
-      seq = pair / pr.heads_kv;
-      kv_head = pair - seq * pr.heads_kv;
-    }
-  } else {
-    const int linear = kSink ? blockIdx.x - p.sinks.ctas : blockIdx.x;
-    if (p.work_list) {
-      const int2 e = p.work_list[linear];
-      seq = e.x;
-      n_block = e.y;
-      kv_head = blockIdx.y;
-      if (seq >= pr.batch) return;
-    } else {
-      const BwdCta cta = bwd_cta_of(p, linear);
-      seq = cta.seq;
-      n_block = cta.n_block;
-      kv_head = cta.head_slot;
-    }
-    if (kSink && p.sinks.rows) {
-      if (!p.work_list) n_block += p.sinks.blocks;  // the fixed-length launch leaves the blocks of the shares out
-      else if (n_block * kBlockN < pr.sink) return;
-    }
-  }
+  const BwdItem item = bwd_item_of<kSink>(p, pr.heads_kv);
+  const int seq = item.seq, n_block = item.n_block, kv_head = item.head_slot, share = item.share;
+  if (seq >= pr.batch) return;
   const SeqInfo s = seq_info(pr, seq);
   const int n0 = n_block * kBlockN;
   if (n0 >= s.lk) return;
@@ -397,12 +357,12 @@ bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CU
           // Rows of the tiles behind the end of a packed sequence belong to the next one or to nobody, so anything may
           // stand there. Their P and dS are 0, but 0 x NaN is not: the K rows (dQ reads them), the Q rows (dK) and the dO
           // rows (dV) become zeros before the barriers that those products wait for. dO is touched once dP^T has read it.
-          if (pr.cu_q && it == 0 && wg == 0 && !key_valid) zero_row<D>(smem_k, r);
+          if (pr.cu_q && it == 0 && wg == 0 && !key_valid) zero_tile_row(smem_k, Cfg::kHalves, Cfg::kPanelBytes, r);
           if (pr.cu_q && qb.limit - qb.col0 < kBlockM) {
             if (!mbar_wait(bar_dp_full, it & 1, wctx, kWaitBwdCompute)) { ok = false; break; }
             if (wg == 0 && r >= qb.limit - qb.col0) {
-              zero_row<D>(smem_q + st * Cfg::kTileBytes, r);
-              zero_row<D>(smem_do, r);
+              zero_tile_row(smem_q + st * Cfg::kTileBytes, Cfg::kHalves, Cfg::kPanelBytes, r);
+              zero_tile_row(smem_do, Cfg::kHalves, Cfg::kPanelBytes, r);
             }
           }
           fence_proxy_async_smem();
@@ -540,11 +500,7 @@ bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CU
         const float mul = is_dv ? 1.f : p.scale;
         const uint32_t t_acc = tmem_base + lane_addr + (is_dv ? Cfg::kTmemDv : Cfg::kTmemDk);
         float* part_row = nullptr;  // a share leaves its sums in FP32, not scaled
-        if (kSink && share >= 0) {
-          const int64_t q0 = pr.cu_q ? s.q0 : (int64_t)seq * pr.seqlen_q;
-          const int64_t slot = q0 / p.sinks.rows + seq + share;
-          part_row = p.sinks.part + ((((slot * pr.heads_kv + kv_head) * p.sinks.blocks + n_block) * 2 + !is_dv) * kBlockN + r) * D;
-        }
+        if (kSink && share >= 0) part_row = sink_part_row(p, s, seq, share, kv_head, n_block, !is_dv, r, D);
         uint4* dst = reinterpret_cast<uint4*>(out + s.batch_coord * bs + (int64_t)(s.k0 + c) * rs + (int64_t)kv_head * hs);
 #pragma unroll
         for (int ch0 = 0; ch0 < D / 32 / kParts; ++ch0) {
@@ -960,7 +916,7 @@ static int sink_share_rows(const b200fa_problem& p, int sink) {
     // One CTA runs per SM, so a launch of two or three waves ends with a full or an almost empty one depending on the number
     // of shares: take the size, up to twice the smallest, with the least product of waves and largest CTA (2 x 4096 tokens,
     // 16/4 heads, window 512: six blocks, two waves instead of five blocks, three waves).
-    const int64_t pairs = (int64_t)p.batch * p.heads_kv, sink_blocks = ceil_div(sink, kBlockN);
+    const int64_t pairs = (int64_t)p.batch * p.heads_kv * (p.head_dim > 128 ? 2 : 1), sink_blocks = ceil_div(sink, kBlockN);
     const int64_t others = pairs * (ceil_div(p.seqlen_k, kBlockN) - sink_blocks), rows = ceil_div(p.seqlen_q, kBlockM);
     int64_t best = 0, best_cost = 0;
     for (int64_t size = blocks; size <= 2 * blocks; ++size) {
@@ -1155,8 +1111,9 @@ static int launch_bwd_d(const b200fa_bwd_args& a, int sink, cudaStream_t stream)
     if (p.sinks.rows) {
       p.sinks.blocks = imin(p.sinks.blocks, ceil_div(bp.seqlen_k, kBlockN));
       p.sinks.per_sequence = ceil_div(bp.seqlen_q, p.sinks.rows);
-      B200FA_REQUIRE((int64_t)p.sinks.per_sequence * bp.batch * bp.heads_kv * p.sinks.blocks < INT_MAX, "too many key blocks for one backward launch");
-      p.sinks.ctas = p.sinks.per_sequence * bp.batch * bp.heads_kv * p.sinks.blocks;
+      const int64_t ctas = (int64_t)p.sinks.per_sequence * bp.batch * bp.heads_kv * kHeadSplit * p.sinks.blocks;
+      B200FA_REQUIRE(ctas < INT_MAX, "too many key blocks for one backward launch");
+      p.sinks.ctas = (int)ctas;
     }
     const int dealt_out = p.sinks.rows ? p.sinks.blocks : 0;  // key blocks in front of those of the launch's main part
     p.n_blocks = ceil_div(bp.seqlen_k, kBlockN) - dealt_out;
@@ -1195,12 +1152,10 @@ static int launch_bwd_d(const b200fa_bwd_args& a, int sink, cudaStream_t stream)
       status = launch_main<D>(a, p, grid, dq_accum, w.rows, stream);
     }
     if (status != B200FA_OK) return status;
-    if constexpr (D <= 128) {
-      if (p.sinks.rows) {
-        const dim3 join((unsigned)(bp.batch * p.sinks.blocks * (kBlockN * D / 4 / 256)), (unsigned)bp.heads_kv);
-        bwd_sink_join_kernel<D><<<join, 256, 0, stream>>>(p);
-        B200FA_CUDA_CHECK(cudaGetLastError());
-      }
+    if (p.sinks.rows) {
+      const dim3 join((unsigned)(bp.batch * p.sinks.blocks * (kBlockN * D / 4 / 256)), (unsigned)bp.heads_kv);
+      bwd_sink_join_kernel<D><<<join, 256, 0, stream>>>(p);
+      B200FA_CUDA_CHECK(cudaGetLastError());
     }
   }
   mark(2, stream);

@@ -24,7 +24,7 @@ constexpr float kDkFixScale = 1099511627776.f;
 struct SinkShares {
   int rows;             // query rows per share, a multiple of 128
   int blocks;           // key blocks per sequence that hold sinks, at most
-  int ctas;             // leading CTAs (grid.x) that hold shares: fixed length over all key heads, packed per key head
+  int ctas;             // leading CTAs (grid.x) that hold shares: fixed length over all head slots, packed per head slot
   int per_sequence;     // fixed length: shares per sequence
   const int2* list;     // packed: (sequence, share) entries
   float* part;          // (slots, heads_kv, blocks, dV and dK, 128, compiled width)
@@ -89,6 +89,55 @@ __device__ __forceinline__ BwdCta bwd_cta_of(const BwdParams& p, int linear) {
   c.seq = g / p.head_slots;
   c.head_slot = g - c.seq * p.head_slots;
   return c;
+}
+
+// What a CTA of a main kernel works on: a key block of a sequence (seq >= batch: nothing), and with kSink, share >= 0, only a
+// share of its query rows (SinkShares).
+struct BwdItem {
+  int seq, n_block, head_slot, share;
+};
+template <bool kSink>
+__device__ __forceinline__ BwdItem bwd_item_of(const BwdParams& p, int head_slots) {
+  BwdItem item{p.prob.batch, 0, 0, -1};
+  if (kSink && blockIdx.x < p.sinks.ctas) {
+    const int entry = blockIdx.x / p.sinks.blocks;
+    item.n_block = blockIdx.x - entry * p.sinks.blocks;
+    if (p.sinks.list) {
+      const int2 e = p.sinks.list[entry];
+      item.seq = e.x;
+      item.share = e.y;
+      item.head_slot = blockIdx.y;
+    } else {
+      const int pair = entry / p.sinks.per_sequence;
+      item.share = entry - pair * p.sinks.per_sequence;
+      item.seq = pair / head_slots;
+      item.head_slot = pair - item.seq * head_slots;
+    }
+    return item;
+  }
+  const int linear = kSink ? blockIdx.x - p.sinks.ctas : blockIdx.x;
+  if (p.work_list) {
+    const int2 e = p.work_list[linear];
+    item.seq = e.x;
+    item.n_block = e.y;
+    item.head_slot = blockIdx.y;
+    if (kSink && p.sinks.rows && item.n_block * kBlockN < p.prob.sink) item.seq = p.prob.batch;  // the shares' part
+  } else {
+    const BwdCta cta = bwd_cta_of(p, linear);
+    item.seq = cta.seq;
+    item.n_block = cta.n_block;
+    item.head_slot = cta.head_slot;
+    if (kSink && p.sinks.rows) item.n_block += p.sinks.blocks;  // the launch leaves the blocks of the shares out
+  }
+  return item;
+}
+
+// Where a share leaves row `row` of its FP32 sums: dV (which = 0) or dK (1), `width` columns.
+__device__ __forceinline__ float* sink_part_row(const BwdParams& p, const SeqInfo& s, int seq, int share, int kv_head, int n_block,
+                                                int which, int row, int width) {
+  const int64_t q0 = p.prob.cu_q ? s.q0 : (int64_t)seq * p.prob.seqlen_q;
+  const int64_t slot = q0 / p.sinks.rows + seq + share;
+  return p.sinks.part + ((((slot * p.prob.heads_kv + kv_head) * p.sinks.blocks + n_block) * 2 + which) * kBlockN + row) * width;
 }
 
 // Main kernel for head_dim in (128, 256]: grid.y = 2 * heads_kv (kv head, half of the head dimension).

@@ -42,26 +42,16 @@ constexpr int kSmemBytes = kOffBars + 192;
 constexpr int kTmemS = 0, kTmemDp = 64, kTmemDv = 128, kTmemDk = 256, kTmemV = 384;
 static_assert(kSmemBytes <= 232448, "shared memory of the head_dim 256 backward kernel exceeds the per-CTA limit");
 
-template <bool kPivot>
+template <bool kPivot, bool kSink>  // kSink: see bwd.cu
 __global__ void __launch_bounds__(kThreads, 1)
 bwd_d256_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                 const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_do,
                 const __grid_constant__ CUtensorMap map_dq, const __grid_constant__ BwdParams p) {
   const Problem& pr = p.prob;
   // ---- work item (uniform over the CTA; exits before any barrier or TMEM allocation)
-  int seq, n_block, head_slot;
-  if (p.work_list) {
-    const int2 e = p.work_list[blockIdx.x];
-    seq = e.x;
-    n_block = e.y;
-    head_slot = blockIdx.y;
-    if (seq >= pr.batch) return;
-  } else {
-    const BwdCta cta = bwd_cta_of(p, blockIdx.x);
-    seq = cta.seq;
-    n_block = cta.n_block;
-    head_slot = cta.head_slot;
-  }
+  const BwdItem item = bwd_item_of<kSink>(p, 2 * pr.heads_kv);
+  const int seq = item.seq, n_block = item.n_block, head_slot = item.head_slot, share = item.share;
+  if (seq >= pr.batch) return;
   const int kv_head = head_slot >> 1;
   const int dh = head_slot & 1;  // half of the head dimension owned by this CTA
   const SeqInfo s = seq_info(pr, seq);
@@ -70,6 +60,12 @@ bwd_d256_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
   const int c1 = imin(n0 + kBlockN, s.lk);
   const int group = pr.heads_q / pr.heads_kv;
   const int64_t stat_base = pr.cu_q ? 0 : (int64_t)seq * pr.seqlen_q;
+  // Walks the query blocks of this CTA: all that see the key block, or those of its share.
+  using Cursor = HalfBlockCursorT<kSink>;
+  auto start_cursor = [&](Cursor& cur) {
+    cur.init(&pr, seq, s, n0, c1);
+    if (kSink && share >= 0) cur.cursor.restrict_to_rows(share * p.sinks.rows, (share + 1) * p.sinks.rows);
+  };
 
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   const uint32_t base = smem_u32(smem_raw);
@@ -124,8 +120,8 @@ bwd_d256_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
   // 64-row query blocks per head (the same for every head of the group).
   int blocks_per_head = 0;
   {
-    HalfBlockCursor cur;
-    cur.init(&pr, seq, s, n0, c1);
+    Cursor cur;
+    start_cursor(cur);
     OtherBlock qb;
     while (cur.next(&qb)) ++blocks_per_head;
   }
@@ -154,8 +150,8 @@ bwd_d256_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       const int head = kv_head * group + g;
       const float* lse_head = p.lse_log2 + (int64_t)head * p.rows;
       const float* dpsum_head = p.dpsum + (int64_t)head * p.rows;
-      HalfBlockCursor cur;
-      cur.init(&pr, seq, s, n0, c1);
+      Cursor cur;
+      start_cursor(cur);
       OtherBlock qb;
       while (cur.next(&qb)) {
         const int st = it & 1;
@@ -315,21 +311,33 @@ bwd_d256_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       }
     }
     for (int g = 0; ok && g < group; ++g) {
-      HalfBlockCursor cur;
-      cur.init(&pr, seq, s, n0, c1);
+      Cursor cur;
+      start_cursor(cur);
       OtherBlock qb;
       while (cur.next(&qb)) {
         const int st = it & 1;
         int qlo = 0, qhi = qb.limit - qb.col0;
         if (qb.banded) {
           if (right >= 0) qlo = imax(0, c - off - right - qb.col0);
-          if (left >= 0) qhi = imin(qhi, c - off + left + 1 - qb.col0);
+          if (left >= 0 && !(kSink && c < pr.sink)) qhi = imin(qhi, c - off + left + 1 - qb.col0);
         }
         if (!key_valid) qhi = 0;
         const bool masked = __any_sync(0xffffffffu, qlo > cb || qhi < cb + kCols);
         // ---- P^T (kept in FP32 registers for dS, stored to TMEM as BF16 for the dV MMA)
         if (!mbar_wait(bar_s_full, it & 1, wctx, kWaitBwdCompute)) { ok = false; break; }
         tc_fence_after();
+        if constexpr (kSink) {  // rows behind the end of a packed sequence become zeros, as in bwd.cu
+          if (pr.cu_q && it == 0 && wg == 0 && !key_valid) zero_tile_row(smem_k, 4, kKvPanel, r);
+          if (pr.cu_q && qb.limit - qb.col0 < kSubM) {
+            if (!mbar_wait(bar_dp_full, it & 1, wctx, kWaitBwdCompute)) { ok = false; break; }
+            if (wg == 0 && r < kSubM && r >= qb.limit - qb.col0) {
+              zero_tile_row(smem_q + st * kStageStride, 4, kQPanel, r);
+              zero_tile_row(smem_do + st * kStageStride, 4, kQPanel, r);
+            }
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+        }
         float pf[kCols];
         tmem_ld16(t_s + cb, reinterpret_cast<uint32_t*>(pf));
         tc_wait_ld();
@@ -435,6 +443,8 @@ bwd_d256_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         const int64_t hs = is_dv ? p.dv_head_stride : p.dk_head_stride;
         const float mul = is_dv ? 1.f : p.scale;
         const uint32_t t_acc = tmem_base + lane_addr + (is_dv ? kTmemDv : kTmemDk);
+        float* part_row = nullptr;  // a share leaves its sums in FP32, not scaled
+        if (kSink && share >= 0) part_row = sink_part_row(p, s, seq, share, kv_head, n_block, !is_dv, r, 256) + dh * 128;
         uint4* dst = reinterpret_cast<uint4*>(out + s.batch_coord * bs + (int64_t)(s.k0 + c) * rs + (int64_t)kv_head * hs + dh * 128);
 #pragma unroll
         for (int ch0 = 0; ch0 < 2; ++ch0) {
@@ -447,7 +457,11 @@ bwd_d256_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
 #pragma unroll
             for (int i = 0; i < 32; ++i) acc[i] = 0;
           }
-          if (key_valid && p.dkv_wide) {  // 32-byte stores: a lane writes whole sectors of its row
+          if (kSink && part_row) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              reinterpret_cast<uint4*>(part_row + 32 * ch)[i] = make_uint4(acc[4 * i], acc[4 * i + 1], acc[4 * i + 2], acc[4 * i + 3]);
+          } else if (key_valid && p.dkv_wide) {  // 32-byte stores: a lane writes whole sectors of its row
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
               uint32_t w[8];
@@ -487,8 +501,8 @@ bwd_d256_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     bool ok = true;
     for (int g = 0; ok && g < group; ++g) {
       const int head = kv_head * group + g;
-      HalfBlockCursor cur;
-      cur.init(&pr, seq, s, n0, c1);
+      Cursor cur;
+      start_cursor(cur);
       OtherBlock qb;
       while (cur.next(&qb)) {
         const int row0 = (int)(stat_base + qb.row) + 2 * kStageRows * dg;
@@ -590,7 +604,7 @@ int launch_bwd_main_d256(const b200fa_bwd_args& a, const BwdParams& p, dim3 grid
     const char* setting = std::getenv("B200FA_BWD_D256_PAIR");
     return setting != nullptr && setting[0] == '1';
   }();
-  if (paired && !p.pivot_key) return launch_bwd_main_d256_pair(a, p, grid, dq_accum, stat_rows, stream);
+  if (paired && !p.pivot_key && p.prob.sink == 0) return launch_bwd_main_d256_pair(a, p, grid, dq_accum, stat_rows, stream);
   const b200fa_problem& bp = a.problem;
   const bool packed = bp.cu_seqlens_q != nullptr;
   const int64_t rows_q = bp.seqlen_q, rows_k = bp.seqlen_k;
@@ -625,17 +639,19 @@ int launch_bwd_main_d256(const b200fa_bwd_args& a, const BwdParams& p, dim3 grid
                                stat_rows * D, D, (int64_t)bp.heads_q * stat_rows * D, 128, kStageRows);
     if (status != B200FA_OK) return status;
   }
-  if (p.pivot_key) {  // pivot gradients requested (b200fa_set_pivot_ds)
-    static bool attribute_set[64] = {false};
-    status = set_dynamic_smem_once(reinterpret_cast<const void*>(&bwd_d256_kernel<true>), kSmemBytes, attribute_set);
-    if (status != B200FA_OK) return status;
-    bwd_d256_kernel<true><<<grid, kThreads, kSmemBytes, stream>>>(map_q, map_k, map_v, map_do, map_dq, p);
-  } else {
-    static bool attribute_set[64] = {false};
-    status = set_dynamic_smem_once(reinterpret_cast<const void*>(&bwd_d256_kernel<false>), kSmemBytes, attribute_set);
-    if (status != B200FA_OK) return status;
-    bwd_d256_kernel<false><<<grid, kThreads, kSmemBytes, stream>>>(map_q, map_k, map_v, map_do, map_dq, p);
+  auto launch = [&](auto kernel, bool (&attribute_set)[64]) -> int {
+    const int set = set_dynamic_smem_once(reinterpret_cast<const void*>(kernel), kSmemBytes, attribute_set);
+    if (set != B200FA_OK) return set;
+    kernel<<<grid, kThreads, kSmemBytes, stream>>>(map_q, map_k, map_v, map_do, map_dq, p);
+    return B200FA_OK;
+  };
+  static bool set_plain[64] = {false}, set_pivot[64] = {false}, set_sink[64] = {false}, set_sink_pivot[64] = {false};
+  if (p.prob.sink > 0) {
+    status = p.pivot_key ? launch(&bwd_d256_kernel<true, true>, set_sink_pivot) : launch(&bwd_d256_kernel<false, true>, set_sink);
+  } else {  // pivot gradients on request (b200fa_set_pivot_ds)
+    status = p.pivot_key ? launch(&bwd_d256_kernel<true, false>, set_pivot) : launch(&bwd_d256_kernel<false, false>, set_plain);
   }
+  if (status != B200FA_OK) return status;
   B200FA_CUDA_CHECK(cudaGetLastError());
   return B200FA_OK;
 }

@@ -27,8 +27,9 @@ constexpr int kStageRows = 16;              // query rows per staging buffer
 constexpr int kStageBytes = kStageRows * 128 * 4;
 
 // Yields the 128-row query blocks of a QueryCursor as 64-row halves (a half past the end of its run is skipped).
-struct HalfBlockCursor {
-  QueryCursor cursor;
+template <bool kSink>
+struct HalfBlockCursorT {
+  QueryCursorT<!kSink, kSink> cursor;
   OtherBlock block;
   int half;
   __device__ void init(const Problem* problem, int seq, const SeqInfo& s, int c0, int c1) {
@@ -50,6 +51,7 @@ struct HalfBlockCursor {
     }
   }
 };
+using HalfBlockCursor = HalfBlockCursorT<false>;
 
 }  // namespace bd256
 

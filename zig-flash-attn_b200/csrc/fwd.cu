@@ -389,26 +389,14 @@ fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CU
           // without having followed the barrier: the scores being present proves the slot's previous use complete.)
           const uint32_t v_index = ring + 2 * tile_blocks + 1;
           if (!mbar_wait(bar_kv_full + 8 * (v_index % NS), (v_index / NS) & 1, wctx, kWaitKvFull)) { ok = false; break; }
-          if (row_in_stage >= kb.limit - kb.col0) {
-            const uint32_t v_row = smem_kv + (v_index % NS) * Cfg::kTileBytes + row_in_stage * 128;
-#pragma unroll 1
-            for (int i = 0; i < Cfg::kHalves * 8; ++i)
-              st_shared_zero16(v_row + (i >> 3) * Cfg::kPanelBytes + (i & 7) * 16);
-          }
+          if (row_in_stage >= kb.limit - kb.col0)
+            zero_tile_row(smem_kv + (v_index % NS) * Cfg::kTileBytes, Cfg::kHalves, Cfg::kPanelBytes, row_in_stage);
           fence_proxy_async_smem();
           __syncwarp();
         }
         auto apply_mask = [&](float2* values, int first_column) {
           if constexpr (kSink) {
-#pragma unroll
-            for (int w = 0; w < 2; ++w) {
-              const uint32_t bits = visible_columns(first_column + 32 * w, lo, hi, sinks);
-#pragma unroll
-              for (int i = 0; i < 16; ++i) {
-                values[16 * w + i].x = (bits & (1u << (2 * i))) ? values[16 * w + i].x : -INFINITY;
-                values[16 * w + i].y = (bits & (2u << (2 * i))) ? values[16 * w + i].y : -INFINITY;
-              }
-            }
+            keep_visible(values, first_column, lo, hi, sinks);
             return;
           }
 #pragma unroll
@@ -957,10 +945,10 @@ int launch_fwd(const b200fa_fwd_args& a, int sink, cudaStream_t stream) {
         const char* value = getenv("B200FA_FWD_D256_PAIR");
         return value && value[0] == '1';
       }();
-      return pair_kernel ? launch_fwd_256_pair(a, stream) : launch_fwd_256(a, stream);
+      return pair_kernel && sink == 0 ? launch_fwd_256_pair(a, stream) : launch_fwd_256(a, sink, stream);
     }
     case 512:
-      return launch_fwd_512(a, stream);
+      return launch_fwd_512(a, sink, stream);
     default:
       set_error("head_dim %d is not supported by the forward kernel (supported: 64, 72, 96, 128, 256, 512)", a.problem.head_dim);
       return B200FA_ERR_UNSUPPORTED;

@@ -80,6 +80,19 @@ __device__ __forceinline__ uint32_t visible_columns(int first, int lo, int hi, i
   return columns_below(hi - first) & (~columns_below(lo - first) | columns_below(sinks - first));
 }
 
+// Scores of 64 columns that start at column `first`, those that are not visible set to -inf (kSink instances).
+__device__ __forceinline__ void keep_visible(float2* values, int first, int lo, int hi, int sinks) {
+#pragma unroll
+  for (int w = 0; w < 2; ++w) {
+    const uint32_t bits = visible_columns(first + 32 * w, lo, hi, sinks);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      values[16 * w + i].x = (bits & (1u << (2 * i))) ? values[16 * w + i].x : -INFINITY;
+      values[16 * w + i].y = (bits & (2u << (2 * i))) ? values[16 * w + i].y : -INFINITY;
+    }
+  }
+}
+
 // Per-row state of the keys that the online softmax sets aside (see row_totals below): `ones` keys, all scoring exactly
 // `apart`, are kept out of the running sum. (Two registers: the softmax warps have none to spare, and a third one for
 // the running maximum of the row cost the masked blocks of causal problems 4 %.)
@@ -275,8 +288,8 @@ int prepare_forward(const b200fa_fwd_args& a, cudaStream_t stream, int head_dim,
 // library, reset by a memset node ahead of the kernel. Launches share a slot only 4096 launches apart (or through a
 // captured graph, which keeps its slot); see the contract at its definition in fwd.cu.
 int acquire_tile_counter(cudaStream_t stream, int** counter);
-int launch_fwd_256(const b200fa_fwd_args& a, cudaStream_t stream);
+int launch_fwd_256(const b200fa_fwd_args& a, int sink, cudaStream_t stream);
 int launch_fwd_256_pair(const b200fa_fwd_args& a, cudaStream_t stream);  // two-CTA variant (fwd_d256_pair.cu)
-int launch_fwd_512(const b200fa_fwd_args& a, cudaStream_t stream);
+int launch_fwd_512(const b200fa_fwd_args& a, int sink, cudaStream_t stream);
 
 }  // namespace b200fa

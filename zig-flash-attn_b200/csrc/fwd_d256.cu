@@ -32,7 +32,9 @@ constexpr int kTmemO = 256;
 static_assert(kSmemBytes <= 232448, "shared memory exceeds the per-CTA limit");
 }  // namespace d256
 
-template <bool kBits>  // false: no visibility bits, the scan of the key cursor is compiled out (see KeyCursorT)
+// kBits = false: no visibility bits, the scan of the key cursor is compiled out (see KeyCursorT); kSink: window attention whose
+// first keys stay visible (b200fa_sink_fwd), see fwd.cu.
+template <bool kBits, bool kSink>
 __global__ void __launch_bounds__(d256::kThreads, 1)
 fwd_d256_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                  const __grid_constant__ CUtensorMap map_v, const __grid_constant__ FwdParams p) {
@@ -89,7 +91,7 @@ fwd_d256_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
 
   // Number of key blocks of a work item (every role needs it to know where the pipeline ends).
   auto count_blocks = [&](const FwdTile& t) {
-    KeyCursorT<kBits> cur;
+    KeyCursorT<kBits, kSink> cur;
     cur.init(&pr, t.seq, t.s, t.m0, imin(t.m0 + kBlockM, t.s.lq));
     OtherBlock kb;
     int n = 0;
@@ -137,7 +139,7 @@ fwd_d256_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         if (!t.valid) continue;
         const int n_blocks = count_blocks(t);
         if (n_blocks == 0) continue;
-        KeyCursorT<kBits> cur_k, cur_v;
+        KeyCursorT<kBits, kSink> cur_k, cur_v;
         cur_k.init(&pr, t.seq, t.s, t.m0, imin(t.m0 + kBlockM, t.s.lq));
         cur_v.init(&pr, t.seq, t.s, t.m0, imin(t.m0 + kBlockM, t.s.lq));
         OtherBlock kb;
@@ -240,7 +242,7 @@ fwd_d256_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       FwdTile t = decode_tile(p, tile, kBlockM);
       if (!t.valid) continue;
       const int row = t.m0 + row_in_tile;
-      KeyCursorT<kBits> cur;
+      KeyCursorT<kBits, kSink> cur;
       cur.init(&pr, t.seq, t.s, t.m0, imin(t.m0 + kBlockM, t.s.lq));
       const int band_lo = cur.band.lo(row), band_hi = cur.band.hi(row);
       float m = -INFINITY, l = 0.f;
@@ -263,8 +265,14 @@ fwd_d256_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
           lo = 0;
           hi = kb.limit - kb.col0;
         }
+        const int sinks = kSink ? pr.sink - kb.col0 : 0;  // columns of this block that hold sinks
+        if (kSink && sinks >= lo) lo = 0;
         const bool masked = __any_sync(0xffffffffu, lo > 0 || hi < kBlockN);
         auto apply_mask = [&](float2* values, int first_column) {
+          if constexpr (kSink) {
+            keep_visible(values, first_column, lo, hi, sinks);
+            return;
+          }
 #pragma unroll
           for (int i = 0; i < 32; ++i) {
             const int c = first_column + 2 * i;
@@ -272,6 +280,18 @@ fwd_d256_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
             values[i].y = (c + 1 >= lo && c + 1 < hi) ? values[i].y : -INFINITY;
           }
         };
+        if (kSink && pr.cu_k && kb.limit - kb.col0 < kBlockN) {
+          // Rows behind the end of a packed sequence may hold anything, and 0 x NaN is not 0: their V rows become zeros
+          // before the products read them (as in fwd.cu). Block n of the launch's blocks of this CTA has its upper half in
+          // V slot 2 n of the ring and its lower half in 2 n + 1; the product of the block before being complete proves the
+          // slots' previous uses complete, which the waits need.
+          if (tile_blocks > 0 && !mbar_wait_warp(bar_pv_done, (blocks - 1) & 1, wctx, kWaitPvDone)) { ok = false; break; }
+          const uint32_t index = 2 * blocks + (row_in_tile < 64);
+          if (!mbar_wait_warp(bar_v_full + 8 * (index % NV), (index / NV) & 1, wctx, kWaitKvFull)) { ok = false; break; }
+          if (row_in_tile >= kb.limit - kb.col0) zero_tile_row(smem_v + (index % NV) * kVBytes, D / 64, kVPanel, row_in_tile & 63);
+          fence_proxy_async_smem();
+          __syncwarp();
+        }
         auto max_of = [&](const float2* values) {
           float a = fmaxf(values[0].x, values[0].y), b = fmaxf(values[1].x, values[1].y);
           float c = fmaxf(values[2].x, values[2].y), d = fmaxf(values[3].x, values[3].y);
@@ -332,7 +352,7 @@ fwd_d256_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         const float2 scale2 = make_float2(scale_log2, scale_log2), shift2 = make_float2(-mc, -mc);
         float sum_counted = 0.f;
         if (counting)  // rare: the block sum without the keys set aside, from the scores still in TMEM
-          sum_counted = sum_without_keys_apart<kBlockN>(top, l, set_apart, block_max, t_s, masked, lo, hi, scale_log2, mc);
+          sum_counted = sum_without_keys_apart<kBlockN, kSink>(top, l, set_apart, block_max, t_s, masked, lo, hi, scale_log2, mc, sinks);
         float2 sum_a = make_float2(0.f, 0.f), sum_b = make_float2(0.f, 0.f);
         // 64 scores -> 64 probabilities (BF16) stored at P columns [first_p_column, first_p_column + 32)
         auto exponentiate = [&](const float2* values, uint32_t first_p_column) {
@@ -436,27 +456,28 @@ fwd_d256_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
   if (warp == 4) tmem_dealloc(tmem_base, 512);
 }
 
-int launch_fwd_256(const b200fa_fwd_args& a, cudaStream_t stream) {
+int launch_fwd_256(const b200fa_fwd_args& a, int sink, cudaStream_t stream) {
   FwdParams p;
   CUtensorMap map_q, map_k, map_v;
   bool nothing_to_do = false;
-  int status = prepare_forward(a, stream, d256::D, kBlockM, kBlockN, &p, &map_q, &map_k, &map_v, &nothing_to_do, 64);
+  int status = prepare_forward(a, stream, d256::D, kBlockM, kBlockN, &p, &map_q, &map_k, &map_v, &nothing_to_do, 64, 0,
+                               sink);
   if (status != B200FA_OK || nothing_to_do) return status;
   int sms = 0;
   status = device_sm_count(&sms);
   if (status != B200FA_OK) return status;
   const int grid = p.num_tiles < sms ? p.num_tiles : sms;
-  if (a.problem.visibility_bits) {
-    static bool attribute_set[64] = {false};
-    status = set_dynamic_smem_once(reinterpret_cast<const void*>(&fwd_d256_kernel<true>), d256::kSmemBytes, attribute_set);
-    if (status != B200FA_OK) return status;
-    fwd_d256_kernel<true><<<grid, d256::kThreads, d256::kSmemBytes, stream>>>(map_q, map_k, map_v, p);
-  } else {
-    static bool attribute_set[64] = {false};
-    status = set_dynamic_smem_once(reinterpret_cast<const void*>(&fwd_d256_kernel<false>), d256::kSmemBytes, attribute_set);
-    if (status != B200FA_OK) return status;
-    fwd_d256_kernel<false><<<grid, d256::kThreads, d256::kSmemBytes, stream>>>(map_q, map_k, map_v, p);
-  }
+  auto launch = [&](auto kernel, bool (&attribute_set)[64]) -> int {
+    const int set = set_dynamic_smem_once(reinterpret_cast<const void*>(kernel), d256::kSmemBytes, attribute_set);
+    if (set != B200FA_OK) return set;
+    kernel<<<grid, d256::kThreads, d256::kSmemBytes, stream>>>(map_q, map_k, map_v, p);
+    return B200FA_OK;
+  };
+  static bool set_bits[64] = {false}, set_plain[64] = {false}, set_sink[64] = {false};
+  status = a.problem.visibility_bits ? launch(&fwd_d256_kernel<true, false>, set_bits)
+           : sink > 0                ? launch(&fwd_d256_kernel<false, true>, set_sink)
+                                     : launch(&fwd_d256_kernel<false, false>, set_plain);
+  if (status != B200FA_OK) return status;
   B200FA_CUDA_CHECK(cudaGetLastError());
   return B200FA_OK;
 }

@@ -356,6 +356,12 @@ __device__ __forceinline__ void st_shared_f32(uint32_t addr, float value) {
 __device__ __forceinline__ void st_shared_zero16(uint32_t addr) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(addr), "r"(0) : "memory");
 }
+// Zeroes row r of a tile in shared memory: `panels` panels of 64 columns, 128 bytes a row (the swizzle stays within a row).
+__device__ __forceinline__ void zero_tile_row(uint32_t tile, int panels, uint32_t panel_bytes, int r) {
+#pragma unroll 1
+  for (int i = 0; i < 8 * panels; ++i) st_shared_zero16(tile + (i >> 3) * panel_bytes + r * 128 + (i & 7) * 16);
+}
+
 __device__ __forceinline__ float ld_shared_f32(uint32_t addr) {
   float value;
   asm volatile("ld.shared.f32 %0, [%1];" : "=f"(value) : "r"(addr) : "memory");

@@ -121,8 +121,8 @@ def flash_attn_sink_func(
     window_size: tuple[int, int] = (-1, -1), deterministic: bool = False, return_attn_probs: bool = False,
 ) -> Tensor | tuple[Tensor, Tensor]:
     """flash_attn_func with a sliding window whose first `sink_size` keys stay visible: query row i sees key j when the
-    right bound (or `causal`) allows it and j is within window_size[0] of it or below sink_size. Head dims 64, 72, 96 and
-    128, forward and backward. Keys and values that no row sees still have to be finite."""
+    right bound (or `causal`) allows it and j is within window_size[0] of it or below sink_size. Head dims as flash_attn_func,
+    forward and backward. Keys and values that no row sees still have to be finite."""
     from ._impl import sink
 
     return sink.flash_attn_sink(q, k, v, None, None, sink_size, softmax_scale, causal, window_size, deterministic, return_attn_probs)
