@@ -189,3 +189,41 @@ def test_ops_have_fake_implementations():
         assert [tuple(t.shape) for t in zigfa.reserve_kv_pages(table, lengths, lengths, refs, 16)] == [(3, 5), (9,)]
         assert zigfa.append_paged_kv(torch.empty(3, 1, 2, 64, dtype=torch.bfloat16), torch.empty(3, 1, 2, 64, dtype=torch.bfloat16),
                                      k, k, table, lengths) is None
+
+
+def test_packed_arguments_have_the_layout_of_the_structures():
+    """The host layer packs the argument structures with `struct`; their sizes and field offsets are those of ctypes."""
+    import struct
+
+    from zigfa._impl import dispatch
+
+    for name, structure in (("fwd", lib.FwdArgs), ("bwd", lib.BwdArgs), ("paged", lib.PagedArgs), ("kv_cache", lib.KvCache),
+                            ("append", lib.AppendArgs), ("pages", lib.PagesArgs)):
+        pack = getattr(dispatch, f"PACK_{name.upper()}")
+        layout = pack.__self__
+
+        def values(fields):  # every scalar of the structure, in order, numbered
+            for _, kind in fields:
+                if hasattr(kind, "_fields_"):
+                    yield from values(kind._fields_)
+                elif hasattr(kind, "_length_"):
+                    yield from [kind._type_] * kind._length_
+                else:
+                    yield kind
+
+        kinds = list(values(structure._fields_))
+        data = pack(*range(1, len(kinds) + 1))
+        assert layout.size <= ctypes.sizeof(structure) < layout.size + 8, name  # a structure may end in padding
+        filled = structure.from_buffer_copy(data.ljust(ctypes.sizeof(structure), b"\0"))
+
+        def read(value):
+            for field, kind in value._fields_:
+                item = getattr(value, field)
+                if hasattr(kind, "_fields_"):
+                    yield from read(item)
+                elif hasattr(kind, "_length_"):
+                    yield from item
+                else:
+                    yield item
+
+        assert list(read(filled)) == list(range(1, len(kinds) + 1)), name

@@ -441,3 +441,32 @@ def test_other_device_than_the_current_one_is_refused_or_used():
         zigfa.flash_attn_paged_func(q.cpu(), k.cpu(), k.cpu(), table.cpu(), lengths.cpu())
     with pytest.raises((ValueError, NotImplementedError)):
         zigfa.copy_kv_pages(k, k, lengths.cpu(), lengths.cpu())
+
+
+def test_ops_pass_the_library_checks_and_compile():
+    utils = ("test_schema", "test_faketensor", "test_aot_dispatch_dynamic")
+    torch.manual_seed(14)
+    table, lengths, refs = ints([[0, 2], [1, 3]]), ints([20, 7]), ints([1, 1, 1, 1, 0, 0])
+    q, k_cache, v_cache = randn(2, 4, 64), randn(6, 16, 2, 64), randn(6, 16, 2, 64)
+    k = randn(2, 1, 2, 64)
+    zigfa.flash_attn_paged_func(q, k_cache, v_cache, table, lengths)
+    for op, arguments in [
+        ("paged_forward", (q, k_cache, v_cache, table, lengths, 0.1, 5, 2)), ("append_kv", (k, k, k_cache, v_cache, table, lengths, None)),
+        ("copy_pages", (k_cache, v_cache, ints([0, -1]), ints([5, -1]))), ("reserve_pages", (table, lengths, lengths, refs, 16)),
+        ("fork_pages", (table, lengths, refs, ints([1, 0, 1]), 16)), ("free_pages", (table, refs, ints([0, 0]), ints([1, 2]))),
+        ("compact_pages", (table, refs)),
+    ]:
+        torch.library.opcheck(getattr(torch.ops.zigfa, op).default, arguments, test_utils=utils)
+
+    def step(q, k, k_cache, v_cache, table, lengths, refs):
+        table, refs = zigfa.reserve_kv_pages(table, lengths, torch.ones_like(lengths), refs, 16)
+        zigfa.append_paged_kv(k, k, k_cache, v_cache, table, lengths)
+        return zigfa.flash_attn_paged_func(q, k_cache, v_cache, table, lengths + 1, window_size=(9, 0), sink_size=2), table, refs
+
+    torch._dynamo.reset()
+    with torch.no_grad():
+        caches = [(k_cache.clone(), v_cache.clone()) for _ in range(2)]
+        want = step(q, k, *caches[0], table, lengths, refs)
+        got = torch.compile(step, fullgraph=True)(q, k, *caches[1], table, lengths, refs)
+    torch._dynamo.reset()
+    assert all(torch.equal(a, b) for a, b in zip(want, got)) and all(torch.equal(a, b) for a, b in zip(*caches))

@@ -198,7 +198,58 @@ def test_head_dims_without_a_kernel_are_refused():
         zigfa.flash_attn_varlen_sink_func(*(randn(64, 2, 64) for _ in range(3)), ints([0, 64]).cpu(), ints([0, 64]).cpu(), 64, 64, 4, window_size=(9, 0))
 
 
+OPCHECK = ("test_schema", "test_autograd_registration", "test_faketensor", "test_aot_dispatch_dynamic")
+
+
 def test_ops_pass_the_library_checks():
     q, k = randn(1, 40, 2, 64), randn(1, 40, 2, 64)
-    torch.library.opcheck(torch.ops.zigfa.sink_forward.default, (q, k, k, None, None, 0.1, 9, 0, 3),
-                          test_utils=("test_schema", "test_faketensor"))
+    arguments = (q, k, k, None, None, 0.1, 9, 0, 3)
+    torch.library.opcheck(torch.ops.zigfa.sink_forward.default, arguments, test_utils=OPCHECK)
+    out, lse = torch.ops.zigfa.sink_forward(*arguments)
+    torch.library.opcheck(torch.ops.zigfa.sink_backward.default, (randn(1, 40, 2, 64), q, k, k, out, lse, *arguments[3:]), test_utils=OPCHECK)
+    cu = ints([0, 10, 40])
+    torch.library.opcheck(torch.ops.zigfa.sink_forward.default, (q[0], k[0], k[0], cu, cu, 0.1, 9, 0, 3), test_utils=OPCHECK)
+
+
+def test_compiled_attention_matches_eager():
+    torch._dynamo.reset()
+    torch.manual_seed(9)
+    q, k, v = (randn(2, 256, h, 128, requires_grad=True) for h in (4, 2, 2))
+
+    def attention(q, k, v):
+        return zigfa.flash_attn_sink_func(q, k, v, 4, causal=True, window_size=(60, -1))
+
+    compiled = torch.compile(attention, fullgraph=True, dynamic=True)
+    out, eager = compiled(q, k, v), attention(q, k, v)
+    dout = randn(*out.shape)
+    got, want = torch.autograd.grad(out, (q, k, v), dout), torch.autograd.grad(eager, (q, k, v), dout)
+    assert torch.equal(out, eager) and torch.equal(got[1], want[1]) and torch.equal(got[2], want[2])
+    assert torch.allclose(got[0].float(), want[0].float(), rtol=2.0**-6, atol=1e-4)
+    torch._dynamo.reset()
+
+
+def test_a_second_derivative_is_refused():
+    q, k, v = (randn(1, 40, 2, 64, requires_grad=True) for _ in range(3))
+    out = zigfa.flash_attn_sink_func(q, k, v, 4, causal=True, window_size=(9, -1))
+    gradient, = torch.autograd.grad(out.float().square().sum(), q, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        gradient.sum().backward()
+
+
+def test_two_streams_at_once():
+    """Calls in flight on two streams share nothing: the same values as one after the other."""
+    torch.manual_seed(10)
+    cu = ints([0, 700, 1500])
+    inputs = [[randn(1500, 8, 128), randn(1500, 2, 128), randn(1500, 2, 128)] for _ in range(2)]
+    calls = [lambda x=x: zigfa.flash_attn_varlen_sink_func(*x, cu, cu, 800, 800, 5, causal=True, window_size=(200, 0)) for x in inputs]
+    want = [call() for call in calls]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(10):
+        for stream, call in zip(streams, calls):
+            with torch.cuda.stream(stream):
+                got.append(call())
+    torch.cuda.synchronize()
+    for i, out in enumerate(got):
+        assert torch.equal(out, want[i % 2])

@@ -147,6 +147,7 @@ class FlashAttnSinkFunc(torch.autograd.Function):
         return out, softmax_lse
 
     @staticmethod
+    @torch.autograd.function.once_differentiable
     def backward(ctx, dout, *unused):
         return *sink_backward(dout, *ctx.saved_tensors, *ctx.options), None, None, None, None, None, None, None
 
