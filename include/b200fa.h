@@ -209,7 +209,7 @@ typedef struct b200fa_paged_args {
   size_t workspace_bytes;
 } b200fa_paged_args;
 
-/* A function of batch, heads_q, heads_kv, head_dim, page_size and max_pages alone. */
+/* A function of batch, heads_q, heads_kv, head_dim, page_size, max_pages, window_left and sink_size alone. */
 size_t b200fa_paged_decode_workspace_bytes(const b200fa_paged_args* args);
 int b200fa_paged_decode(const b200fa_paged_args* args, void* stream);
 /* Host twin of the key selection: the keys that the new token of a sequence of `length` keys sees, `capacity` being

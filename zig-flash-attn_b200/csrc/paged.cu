@@ -568,22 +568,29 @@ struct PagedShape {
   size_t o_bytes, ml_bytes, cut_bytes;
   size_t total() const { return o_bytes + ml_bytes + cut_bytes; }
 };
-// Pairs of at most so many steps, five or six per warp of a block, are not cut: up to there the plan and the join kernel take
-// longer than the steps of one block. One sequence, 32/8 heads of 128: 256 keys 6.3 us uncut and 9.1 us cut, 512 keys 9.1
-// and 8.9, 1024 keys 13.6 and 9.4; on the host 16 us a call and 20.
-static int uncut_steps(int head_dim) { return head_dim <= 128 ? 32 : 16; }
+// Pairs of at most so many steps are not cut: up to there the plan and the join kernel take longer than the steps of one
+// block, 5 us on the GPU and as much on the host. One sequence, 32/8 heads of 128 (8 pairs): 256 keys 6.3 us uncut and 9.1
+// cut, 512 keys 9.1 and 8.9, 1024 keys 13.6 and 9.4. With so many pairs that most SMs have one, longer ones need no cut
+// either: 128 pairs of 1024 keys 16.5 and 21.7, of 0 to 1500 keys 19.9 and 22.2, of 0 to 2048 keys 25.0 and 24.6.
+static int uncut_steps(int head_dim, int64_t pairs) { return (head_dim <= 128 ? 32 : 16) * (pairs >= 100 ? 3 : 1); }
 static PagedShape paged_shape(const b200fa_paged_args& a) {
   PagedShape s;
   const int group = a.heads_q / a.heads_kv;
   s.tiles = paged_tiles(a.head_dim, group);
   s.chunks = (group + 8 * s.tiles - 1) / (8 * s.tiles);
-  const int64_t most_steps = ((int64_t)a.max_pages * a.page_size + kPagedStep - 1) / kPagedStep + 1;
+  const int64_t most_steps = ((int64_t)a.max_pages * a.page_size + kPagedStep - 1) / kPagedStep;
   const int blocks_per_sm = a.head_dim <= 256 ? 2 : 1;
   const int64_t most_work = most_steps * a.batch * a.heads_kv * s.chunks, wanted = (most_work + kMinSteps - 1) / kMinSteps;
   s.ranges = wanted < blocks_per_sm * kPagedSms ? (int)wanted : blocks_per_sm * kPagedSms;
   s.o_bytes = s.ml_bytes = s.cut_bytes = 0;
-  if (most_steps <= uncut_steps(a.head_dim) + 1) {
-    const int64_t pairs = (int64_t)a.batch * a.heads_kv * s.chunks;
+  const int64_t pairs = (int64_t)a.batch * a.heads_kv * s.chunks;
+  // steps of a pair, at most: a window bounds them whatever the table holds
+  int64_t pair_steps = most_steps;
+  if (a.window_left >= 0) {
+    const int64_t seen = ((int64_t)a.window_left + kPagedStep) / kPagedStep + 1 + ((int64_t)a.sink_size + kPagedStep - 1) / kPagedStep;
+    pair_steps = seen < most_steps ? seen : most_steps;
+  }
+  if (pair_steps <= uncut_steps(a.head_dim, pairs)) {
     s.ranges = pairs < blocks_per_sm * kPagedSms ? (int)pairs : blocks_per_sm * kPagedSms;
     return s;
   }

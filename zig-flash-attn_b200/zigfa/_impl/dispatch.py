@@ -69,6 +69,14 @@ def on_device(index, function, *arguments):
 stream_of = torch._C._cuda_getCurrentRawStream
 
 
+def readable(tensor):
+    """`tensor`, or a contiguous copy where the kernels cannot address it (ops.kernel_ready) -- of three dimensions or more."""
+    stride = tensor.stride()
+    if stride[-1] == 1 and not (stride[0] | stride[1] | stride[-2]) & 7 and not tensor.data_ptr() & 15:
+        return tensor
+    return tensor.clone(memory_format=torch.contiguous_format)
+
+
 def refuse_gradients(what, *tensors):
     if torch.is_grad_enabled():
         for tensor in tensors:

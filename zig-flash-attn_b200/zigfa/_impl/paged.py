@@ -15,8 +15,8 @@ import torch
 
 from . import lib as _lib
 from . import ops
-from .dispatch import (PACK_APPEND, PACK_KV_CACHE, PACK_PAGED, PACK_PAGES, define, entry, on_device, refuse_gradients,
-                       stream_of)
+from .dispatch import (PACK_APPEND, PACK_KV_CACHE, PACK_PAGED, PACK_PAGES, define, entry, on_device, readable,
+                       refuse_gradients, stream_of)
 
 BF16, INT32 = torch.bfloat16, torch.int32
 
@@ -136,8 +136,9 @@ def _is_cache(k_cache, v_cache):
 
 
 @functools.lru_cache(maxsize=4096)
-def _paged_workspace(batch, heads_q, heads_kv, head_dim, page_size, max_pages):
-    args = _lib.PagedArgs(batch=batch, heads_q=heads_q, heads_kv=heads_kv, head_dim=head_dim, page_size=page_size, max_pages=max_pages)
+def _paged_workspace(batch, heads_q, heads_kv, head_dim, page_size, max_pages, window_left, sink_size):
+    args = _lib.PagedArgs(batch=batch, heads_q=heads_q, heads_kv=heads_kv, head_dim=head_dim, page_size=page_size,
+                          max_pages=max_pages, window_left=window_left, sink_size=sink_size)
     return _lib.library().b200fa_paged_decode_workspace_bytes(args)
 
 
@@ -155,11 +156,10 @@ def _paged_forward(q, k_cache, v_cache, block_table, cache_seqlens, softmax_scal
     max_pages = block_table.shape[1]
     if not cache_seqlens.is_contiguous():
         cache_seqlens = cache_seqlens.contiguous()
-    if not ops.kernel_ready(q):
-        q = q.clone(memory_format=torch.contiguous_format)
+    q = readable(q)
     out = torch.empty_like(q, memory_format=torch.contiguous_format)
     softmax_lse = q.new_empty((batch, heads_q), dtype=torch.float32)
-    nbytes = _paged_workspace(batch, heads_q, heads_kv, head_dim, page_size, max_pages)
+    nbytes = _paged_workspace(batch, heads_q, heads_kv, head_dim, page_size, max_pages, window_left, sink_size)
     workspace = q.new_empty((nbytes,), dtype=torch.uint8) if nbytes else None
     q_stride, k_stride, v_stride = q.stride(), k_cache.stride(), v_cache.stride()
     packed = PACK_PAGED(
@@ -191,7 +191,7 @@ def _append_kv(k, v, k_cache, v_cache, block_table, cache_seqlens, cu_seqlens):
         and device == v.get_device() == k_cache.get_device() == v_cache.get_device() == block_table.get_device() == cache_seqlens.get_device()
     ):
         check_append(k, v, k_cache, v_cache, block_table, cache_seqlens, cu_seqlens)
-    k, v, cache_seqlens, cu_seqlens = ops.readable(k), ops.readable(v), ops._contiguous_int(cache_seqlens), ops._contiguous_int(cu_seqlens)
+    k, v, cache_seqlens, cu_seqlens = readable(k), readable(v), ops._contiguous_int(cache_seqlens), ops._contiguous_int(cu_seqlens)
     num_pages, page_size, heads, head_dim = k_cache.shape
     arguments = PACK_APPEND(
         num_pages, page_size, heads, head_dim, k_cache.data_ptr(), v_cache.data_ptr(), *k_cache.stride()[:3],

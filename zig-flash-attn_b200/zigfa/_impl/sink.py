@@ -10,7 +10,7 @@ import torch
 
 from . import lib as _lib
 from . import ops
-from .dispatch import PACK_BWD, PACK_FWD, define, entry, on_device, stream_of
+from .dispatch import PACK_BWD, PACK_FWD, define, entry, on_device, readable, stream_of
 
 BF16, INT32 = torch.bfloat16, torch.int32
 
@@ -67,7 +67,7 @@ def _forward(q, k, v, cu_seqlens_q, cu_seqlens_k, softmax_scale, window_left, wi
     if not _fits(q, k, v, cu_seqlens_q, cu_seqlens_k):
         _check_tensors(q, k, v, cu_seqlens_q, cu_seqlens_k, ops.FORWARD)
     packed, device = cu_seqlens_q is not None, q.get_device()
-    q, k, v = ops.readable(q), ops.readable(k), ops.readable(v)
+    q, k, v = readable(q), readable(k), readable(v)
     out = torch.empty_like(q, memory_format=torch.contiguous_format)
     softmax_lse = q.new_empty(ops.lse_shape(q, packed), dtype=torch.float32)
     if packed:
@@ -106,20 +106,21 @@ def _backward(dout, q, k, v, out, softmax_lse, cu_seqlens_q, cu_seqlens_k, softm
     ):
         ops.check_same_device(q, dout=dout, out=out, softmax_lse=softmax_lse)
         ops.check_backward_operands(dout, q, k, v, out, softmax_lse, q, k, v, packed)
-    dout, q, k, v, out = ops.readable(dout), ops.readable(q), ops.readable(k), ops.readable(v), ops.readable(out)
-    softmax_lse = softmax_lse.contiguous()
-    dq, dk, dv = (torch.empty_like(x, memory_format=torch.contiguous_format) for x in (q, k, v))
+    dout, q, k, v, out, softmax_lse = readable(dout), readable(q), readable(k), readable(v), readable(out), softmax_lse.contiguous()
+    dq = torch.empty_like(q, memory_format=torch.contiguous_format)
+    dk = torch.empty_like(k, memory_format=torch.contiguous_format)
+    dv = torch.empty_like(v, memory_format=torch.contiguous_format)
     if packed:
         cu_seqlens_q, cu_seqlens_k = ops._contiguous_int(cu_seqlens_q), ops._contiguous_int(cu_seqlens_k)
     problem = _problem(q, k, cu_seqlens_q, window_left, window_right)
     nbytes = _workspace_bytes("bwd", sink_size, packed, *problem)
     workspace = q.new_empty((max(nbytes, 1),), dtype=torch.uint8)
-    tensors = (q, k, v, out, dout, softmax_lse, dq, dk, dv)
-    strides = [stride for tensor in (q, k, v, out, dout, dq, dk, dv) for stride in _strides(tensor, packed)]
-    lse_stride = softmax_lse.stride()
+    lse_stride, stride_dk = softmax_lse.stride(), _strides(dk, packed)
     arguments = PACK_BWD(
         *problem, softmax_scale, cu_seqlens_q.data_ptr() if packed else 0, cu_seqlens_k.data_ptr() if packed else 0, 0, 0, 0, 0, 0,
-        *(tensor.data_ptr() for tensor in tensors), *strides, 0 if packed else lse_stride[0], lse_stride[-2],
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), dout.data_ptr(), softmax_lse.data_ptr(), dq.data_ptr(),
+        dk.data_ptr(), dv.data_ptr(), *_strides(q, packed), *_strides(k, packed), *_strides(v, packed), *_strides(out, packed),
+        *_strides(dout, packed), *_strides(dq, packed), *stride_dk, *stride_dk, 0 if packed else lse_stride[0], lse_stride[-2],
         workspace.data_ptr(), nbytes,
     )
     on_device(device, entry("b200fa_sink_bwd", ctypes.c_int32, ctypes.c_void_p), arguments, sink_size, stream_of(device))
