@@ -761,15 +761,54 @@ struct PivotFix {
   int group;                     // query heads per key head
 };
 
+// dK and dV of the key blocks whose work was dealt out in shares: the sum of the shares' parts, in their order. A
+// block of 256 threads per (key block of a sequence, key head, 256 / (D / 4) rows), further blocks of the postprocess
+// launch; a thread adds four columns of dV and of dK.
+template <int D>
+__device__ __forceinline__ void join_sink_shares(const BwdParams& p, int block, int kv_head) {
+  constexpr int kQuads = D / 4, kRows = 256 / kQuads;
+  const Problem& pr = p.prob;
+  constexpr int per_block = kBlockN / kRows;
+  const int group = block / per_block, r = (block - group * per_block) * kRows + threadIdx.x / kQuads;
+  const int seq = group / p.sinks.blocks, n_block = group - seq * p.sinks.blocks;
+  const int column = 4 * (threadIdx.x % kQuads);
+  const SeqInfo s = seq_info(pr, seq);
+  const int c = n_block * kBlockN + r;
+  if (n_block * kBlockN >= pr.sink || c >= s.lk || column >= p.head_dim) return;
+  const int64_t q0 = pr.cu_q ? s.q0 : (int64_t)seq * pr.seqlen_q, slot0 = q0 / p.sinks.rows + seq;
+  const int shares = ceil_div(s.lq, p.sinks.rows);
+  const int64_t tile = (int64_t)kBlockN * D, stride = (int64_t)pr.heads_kv * p.sinks.blocks * 2 * tile;
+  const float* part = p.sinks.part + slot0 * stride + (((int64_t)kv_head * p.sinks.blocks + n_block) * 2) * tile + r * D + column;
+  float4 dv = make_float4(0.f, 0.f, 0.f, 0.f), dk = dv;
+#pragma unroll 4
+  for (int i = 0; i < shares; ++i) {
+    const float4 a = *reinterpret_cast<const float4*>(part + i * stride);
+    const float4 b = *reinterpret_cast<const float4*>(part + i * stride + tile);
+    dv.x += a.x, dv.y += a.y, dv.z += a.z, dv.w += a.w;
+    dk.x += b.x, dk.y += b.y, dk.z += b.z, dk.w += b.w;
+  }
+  const int64_t row = s.k0 + c;
+  *reinterpret_cast<uint2*>(p.dv + s.batch_coord * p.dv_batch_stride + row * p.dv_row_stride + kv_head * p.dv_head_stride + column) =
+      make_uint2(pack_bf16x2(dv.x, dv.y), pack_bf16x2(dv.z, dv.w));
+  *reinterpret_cast<uint2*>(p.dk + s.batch_coord * p.dk_batch_stride + row * p.dk_row_stride + kv_head * p.dk_head_stride + column) =
+      make_uint2(pack_bf16x2(dk.x * p.scale, dk.y * p.scale), pack_bf16x2(dk.z * p.scale, dk.w * p.scale));
+}
+
 // dq = bf16(scale * (dq_accum + dS_pivot * K[pivot])) for valid rows, and the pivot term dS_pivot * scale * Q[row] of
 // dK into the FP32 side buffer (reference zig/flash_bwd_postprocess.zig:139-347). dS_pivot = -pivot_sum / kPivotSumScale:
 // the dS of a row add up to zero, so the one the main kernel left out is minus the sum of the others, without the
 // cancellation of P (dP - D) for P near 1 (reference zig/fragments.zig:23-30).
-template <int D>
+// kSink: blocks at and behind `row_blocks` (grid.x) join the shares of the key blocks that hold sinks.
+template <int D, bool kSink>
 __global__ void __launch_bounds__(256) bwd_postprocess_kernel(const float* __restrict__ dq_accum, RowMap map, float scale,
                                                               __nv_bfloat16* __restrict__ dq, int64_t dq_bs,
-                                                              int64_t dq_rs, int64_t dq_hs, PivotFix fix) {
+                                                              int64_t dq_rs, int64_t dq_hs, PivotFix fix, int row_blocks,
+                                                              const __grid_constant__ BwdParams p) {
   using P = PrePost<D>;
+  if (kSink && (int)blockIdx.x >= row_blocks) {
+    if ((int)blockIdx.y < p.prob.heads_kv) join_sink_shares<D>(p, blockIdx.x - row_blocks, blockIdx.y);
+    return;
+  }
   const int lane = threadIdx.x & 31;
   const int sub = lane % P::kLanesPerRow;
   const int64_t row = (int64_t)blockIdx.x * P::kRowsPerBlock + (threadIdx.x >> 5) * P::kRowsPerWarp + lane / P::kLanesPerRow;
@@ -846,38 +885,6 @@ __global__ void __launch_bounds__(256) bwd_fix_dk_kernel(const float* __restrict
     packed.w = pack_bf16x2(__uint_as_float(old.w << 16) + b.z * unscale, __uint_as_float(old.w & 0xffff0000u) + b.w * unscale);
     *dst = packed;
   }
-}
-
-// dK and dV of the key blocks whose work was dealt out in shares: the sum of the shares' parts, in their order. One block of
-// 256 threads per (key block of a sequence, key head, 256 / (D / 4) rows); a thread adds four columns of dV and of dK.
-template <int D>
-__global__ void __launch_bounds__(256) bwd_sink_join_kernel(const __grid_constant__ BwdParams p) {
-  constexpr int kQuads = D / 4, kRows = 256 / kQuads;
-  const Problem& pr = p.prob;
-  const int per_block = kBlockN / kRows;
-  const int group = blockIdx.x / per_block, r = (blockIdx.x - group * per_block) * kRows + threadIdx.x / kQuads;
-  const int seq = group / p.sinks.blocks, n_block = group - seq * p.sinks.blocks, kv_head = blockIdx.y;
-  const int column = 4 * (threadIdx.x % kQuads);
-  const SeqInfo s = seq_info(pr, seq);
-  const int c = n_block * kBlockN + r;
-  if (n_block * kBlockN >= pr.sink || c >= s.lk || column >= p.head_dim) return;
-  const int64_t q0 = pr.cu_q ? s.q0 : (int64_t)seq * pr.seqlen_q, slot0 = q0 / p.sinks.rows + seq;
-  const int shares = ceil_div(s.lq, p.sinks.rows);
-  const int64_t tile = (int64_t)kBlockN * D, stride = (int64_t)pr.heads_kv * p.sinks.blocks * 2 * tile;
-  const float* part = p.sinks.part + slot0 * stride + (((int64_t)kv_head * p.sinks.blocks + n_block) * 2) * tile + r * D + column;
-  float4 dv = make_float4(0.f, 0.f, 0.f, 0.f), dk = dv;
-#pragma unroll 4
-  for (int i = 0; i < shares; ++i) {
-    const float4 a = *reinterpret_cast<const float4*>(part + i * stride);
-    const float4 b = *reinterpret_cast<const float4*>(part + i * stride + tile);
-    dv.x += a.x, dv.y += a.y, dv.z += a.z, dv.w += a.w;
-    dk.x += b.x, dk.y += b.y, dk.z += b.z, dk.w += b.w;
-  }
-  const int64_t row = s.k0 + c;
-  *reinterpret_cast<uint2*>(p.dv + s.batch_coord * p.dv_batch_stride + row * p.dv_row_stride + kv_head * p.dv_head_stride + column) =
-      make_uint2(pack_bf16x2(dv.x, dv.y), pack_bf16x2(dv.z, dv.w));
-  *reinterpret_cast<uint2*>(p.dk + s.batch_coord * p.dk_batch_stride + row * p.dk_row_stride + kv_head * p.dk_head_stride + column) =
-      make_uint2(pack_bf16x2(dk.x * p.scale, dk.y * p.scale), pack_bf16x2(dk.z * p.scale, dk.w * p.scale));
 }
 
 // ---------------------------------------------------------------------------------------------- host side
@@ -1095,14 +1102,13 @@ static int launch_bwd_d(const b200fa_bwd_args& a, int sink, cudaStream_t stream)
   }
   if (run_main && packed) {
     const int32_t* other = bp.cu_visible_q ? bp.cu_visible_q : bp.cu_seqlens_q;
-    int status = b200fa_work_list(bp.cu_seqlens_k, other, bp.batch, kBlockN, 0, (int32_t)w.entries,
-                                  reinterpret_cast<int32_t*>(ws + w.work_list), stream);
+    WorkLists lists{{bp.cu_seqlens_k, bp.cu_seqlens_q}, {other, bp.cu_seqlens_q}, {kBlockN, p.sinks.rows}, {0, 0},
+                    {(int)w.entries, (int)w.sink_entries},
+                    {reinterpret_cast<int2*>(ws + w.work_list), reinterpret_cast<int2*>(ws + w.sink_list)}};
+    const int status = launch_work_lists(lists, p.sinks.rows ? 2 : 1, bp.batch, stream);
     if (status != B200FA_OK) return status;
     p.work_list = reinterpret_cast<const int2*>(ws + w.work_list);
     if (p.sinks.rows) {
-      status = b200fa_work_list(bp.cu_seqlens_q, bp.cu_seqlens_q, bp.batch, p.sinks.rows, 0, (int32_t)w.sink_entries,
-                                reinterpret_cast<int32_t*>(ws + w.sink_list), stream);
-      if (status != B200FA_OK) return status;
       p.sinks.list = reinterpret_cast<const int2*>(ws + w.sink_list);
       p.sinks.ctas = (int)w.sink_entries * p.sinks.blocks;
     }
@@ -1152,11 +1158,6 @@ static int launch_bwd_d(const b200fa_bwd_args& a, int sink, cudaStream_t stream)
       status = launch_main<D>(a, p, grid, dq_accum, w.rows, stream);
     }
     if (status != B200FA_OK) return status;
-    if (p.sinks.rows) {
-      const dim3 join((unsigned)(bp.batch * p.sinks.blocks * (kBlockN * D / 4 / 256)), (unsigned)bp.heads_kv);
-      bwd_sink_join_kernel<D><<<join, 256, 0, stream>>>(p);
-      B200FA_CUDA_CHECK(cudaGetLastError());
-    }
   }
   mark(2, stream);
 
@@ -1175,8 +1176,12 @@ static int launch_bwd_d(const b200fa_bwd_args& a, int sink, cudaStream_t stream)
       fix.key_rows = bp.seqlen_k;
       fix.group = bp.heads_q / bp.heads_kv;
     }
-    bwd_postprocess_kernel<D><<<post, 256, 0, stream>>>(dq_accum, map, bp.softmax_scale, static_cast<__nv_bfloat16*>(a.dq),
-                                                        packed ? 0 : a.dq_stride[0], a.dq_stride[1], a.dq_stride[2], fix);
+    const int row_blocks = (int)post.x;
+    const bool join = run_main && p.sinks.rows > 0;
+    if (join) post.x += (unsigned)(bp.batch * p.sinks.blocks * (kBlockN * D / 4 / 256));
+    auto* kernel = join ? &bwd_postprocess_kernel<D, true> : &bwd_postprocess_kernel<D, false>;
+    kernel<<<post, 256, 0, stream>>>(dq_accum, map, bp.softmax_scale, static_cast<__nv_bfloat16*>(a.dq),
+                                     packed ? 0 : a.dq_stride[0], a.dq_stride[1], a.dq_stride[2], fix, row_blocks, p);
     B200FA_CUDA_CHECK(cudaGetLastError());
     if (pivots && run_main) {
       const int64_t items = w.key_rows * bp.heads_kv * (D / 8);

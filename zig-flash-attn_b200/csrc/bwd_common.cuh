@@ -19,7 +19,7 @@ constexpr float kDkFixScale = 1099511627776.f;
 
 // Sinks make the first key blocks of a sequence heavy: every query row sees them, while the others are seen by a window of
 // rows. Their work is therefore dealt out in shares of `rows` query rows, one CTA each (rows = 0: it is not), which start
-// first and leave FP32 parts of dK and dV, added up in order by bwd_sink_join_kernel. Share i of a sequence that starts at
+// first and leave FP32 parts of dK and dV, added up in order by the postprocess launch. Share i of a sequence that starts at
 // query row q0 has the slot q0 / rows + sequence + i: no two shares have the same, and there are rows_total / rows + batch.
 struct SinkShares {
   int rows;             // query rows per share, a multiple of 128

@@ -16,9 +16,13 @@ constexpr int kListThreads = 1024;
 constexpr uint32_t kClasses = 128;
 
 // ------------------------------------------------------------------------------------------------ work list
-__global__ void __launch_bounds__(kListThreads, 1)
-work_list_kernel(const int32_t* __restrict__ cu, const int32_t* __restrict__ cu_other, int batch, int block_rows,
-                 int descending, int num_entries, int2* __restrict__ table) {
+// One block per list.
+__global__ void __launch_bounds__(kListThreads, 1) work_list_kernel(const __grid_constant__ WorkLists lists, int batch) {
+  const int32_t* __restrict__ cu = lists.cu[blockIdx.x];
+  const int32_t* __restrict__ cu_other = lists.cu_other[blockIdx.x];
+  const int block_rows = lists.block_rows[blockIdx.x], descending = lists.descending[blockIdx.x];
+  const int num_entries = lists.num_entries[blockIdx.x];
+  int2* __restrict__ table = lists.table[blockIdx.x];
   __shared__ uint32_t keys[kListThreads];
   __shared__ int order[kListThreads];
   __shared__ int count[kListThreads];
@@ -73,6 +77,12 @@ work_list_kernel(const int32_t* __restrict__ cu, const int32_t* __restrict__ cu_
     __syncthreads();  // the shared arrays may be overwritten
   }
   for (int entry = written + tid; entry < num_entries; entry += kListThreads) table[entry] = make_int2(batch, 0);
+}
+
+int launch_work_lists(const WorkLists& lists, int count, int batch, cudaStream_t stream) {
+  work_list_kernel<<<(unsigned)count, kListThreads, 0, stream>>>(lists, batch);
+  B200FA_CUDA_CHECK(cudaGetLastError());
+  return B200FA_OK;
 }
 
 // ------------------------------------------------------------------------------------------------ metadata
@@ -205,10 +215,10 @@ int b200fa_work_list(const int32_t* cu_seqlens, const int32_t* cu_seqlens_other,
   if (num_entries == 0) return B200FA_OK;
   B200FA_REQUIRE(cu_seqlens && cu_seqlens_other && table, "work list: null pointer");
   B200FA_REQUIRE(reinterpret_cast<uintptr_t>(table) % 8 == 0, "work list: table must be 8-byte aligned");
-  work_list_kernel<<<1, kListThreads, 0, static_cast<cudaStream_t>(stream)>>>(
-      cu_seqlens, cu_seqlens_other, batch, block_rows, descending, num_entries, reinterpret_cast<int2*>(table));
-  B200FA_CUDA_CHECK(cudaGetLastError());
-  return B200FA_OK;
+  WorkLists lists{};
+  lists.cu[0] = cu_seqlens, lists.cu_other[0] = cu_seqlens_other, lists.block_rows[0] = block_rows;
+  lists.descending[0] = descending, lists.num_entries[0] = num_entries, lists.table[0] = reinterpret_cast<int2*>(table);
+  return launch_work_lists(lists, 1, batch, static_cast<cudaStream_t>(stream));
 }
 
 int b200fa_work_list_host(const int32_t* cu_seqlens, const int32_t* cu_seqlens_other, int32_t batch, int32_t block_rows,
