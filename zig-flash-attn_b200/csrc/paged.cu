@@ -506,12 +506,12 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
 // Joins the parts of the pairs that were cut: out = sum w o / sum w l, w = exp2(m - max m). One block per (range, query head
 // of a chunk); the one of the pair's second range does the work. Its threads form groups of one thread per four columns,
 // group i takes the parts i, i + groups, ... in this order, and the groups are joined in order at the end, so the result
-// does not depend on the schedule. The blocks start under the last ranges and wait for them.
+// does not depend on the schedule. The blocks start under the last ranges and wait for them. `columns` = 8 * NT.
 constexpr int kJoinThreads = 256;
-__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_constant__ PagedParams p) {
+__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_constant__ PagedParams p, int columns) {
   __shared__ float4 group_o[kJoinThreads];
   __shared__ float2 group_ml[kJoinThreads];
-  const int quads = p.head_dim / 4, groups = kJoinThreads / quads, columns = gridDim.y;
+  const int quads = p.head_dim / 4, groups = kJoinThreads / quads;
   const int group = threadIdx.x / quads, quad = threadIdx.x - group * quads, column = blockIdx.y, range = blockIdx.x + 1;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int4 cut = p.cut[range];  // sequence, chunk, first range, last range
@@ -714,12 +714,13 @@ int b200fa_paged_decode(const b200fa_paged_args* a, void* stream) {
     attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attribute.val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t config = {};
-    config.gridDim = dim3((unsigned)shape.ranges - 1, 8u * shape.tiles);
+    const int columns = 8 * shape.tiles;
+    config.gridDim = dim3((unsigned)shape.ranges - 1, (unsigned)(p.group < columns ? p.group : columns));
     config.blockDim = dim3(kJoinThreads);
     config.stream = s;
     config.attrs = &attribute;
     config.numAttrs = 1;
-    B200FA_CUDA_CHECK(cudaLaunchKernelEx(&config, paged_join_kernel, p));
+    B200FA_CUDA_CHECK(cudaLaunchKernelEx(&config, paged_join_kernel, p, columns));
   }
   return B200FA_OK;
 }

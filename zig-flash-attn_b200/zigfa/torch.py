@@ -134,7 +134,8 @@ def flash_attn_varlen_sink_func(
     deterministic: bool = False, return_attn_probs: bool = False,
 ) -> Tensor | tuple[Tensor, Tensor]:
     """flash_attn_sink_func for packed batches (flash_attn_varlen_func): the first `sink_size` keys of every sequence stay
-    visible to its own rows. Rows behind the last sequence are neither read nor written, whatever they hold."""
+    visible to its own rows. Rows behind the last sequence are left as they are, and what they hold (NaN included) has no
+    effect on any result."""
     from ._impl import sink
 
     return sink.flash_attn_sink(q, k, v, cu_seqlens_q, cu_seqlens_k, sink_size, softmax_scale, causal, window_size, deterministic, return_attn_probs)
