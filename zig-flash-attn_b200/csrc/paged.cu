@@ -569,7 +569,7 @@ struct PagedShape {
   size_t total() const { return o_bytes + ml_bytes + cut_bytes; }
 };
 // Pairs of at most so many steps are not cut: up to there the plan and the join kernel take longer than the steps of one
-// block, 5 us on the GPU and as much on the host. One sequence, 32/8 heads of 128 (8 pairs): 256 keys 6.3 us uncut and 9.1
+// block: 3 to 5 us on the GPU, 4 on the host. One sequence, 32/8 heads of 128 (8 pairs): 256 keys 6.3 us uncut and 9.1
 // cut, 512 keys 9.1 and 8.9, 1024 keys 13.6 and 9.4. With so many pairs that most SMs have one, longer ones need no cut
 // either: 128 pairs of 1024 keys 16.5 and 21.7, of 0 to 1500 keys 19.9 and 22.2, of 0 to 2048 keys 25.0 and 24.6.
 static int uncut_steps(int head_dim, int64_t pairs) { return (head_dim <= 128 ? 32 : 16) * (pairs >= 100 ? 3 : 1); }

@@ -1,9 +1,9 @@
 """Short way from the public functions to the C entries, for operators that are called once per layer and token.
 
 An operator is registered with the dispatcher (schema, CUDA implementation, fake implementation for tracing), but plain
-tensors in eager mode go straight to the implementation: the dispatcher's way through Python costs 6 us a call, and the
-wrapper of `torch.library.custom_op` several times that, more than the small kernels take. Argument structures are packed
-with `struct` (1 us for forty fields) in the layout of include/b200fa.h.
+tensors in eager mode go straight to the implementation, which the host needs for calls that take it longer than the GPU:
+appending one token to 64 sequences 11.3 us instead of 13.7, paged attention of one sequence 15.2 instead of 18.5.
+Argument structures are packed with `struct` (0.3 us for 30 fields) in the layout of include/b200fa.h.
 """
 from __future__ import annotations
 
