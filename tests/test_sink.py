@@ -2,6 +2,7 @@
 the host layer and the C entries refuse."""
 import ctypes
 import itertools
+import time
 
 import pytest
 import torch
@@ -126,3 +127,20 @@ def test_the_reference_gradients_match_differences():
         assert torch.autograd.gradcheck(loss, (q, k, v))
         for name, gradient in zip(("dq", "dk", "dv"), torch.autograd.grad(loss(q, k, v), (q, k, v))):
             assert torch.allclose(results[name][0], gradient, rtol=1e-9, atol=1e-12), name
+
+
+@pytest.mark.parametrize("seqlen", [512, 4096, 131072])
+def test_plan_of_a_window_wider_than_any_sequence_is_quick(seqlen):
+    # A bound of 2^30 keys, which the host layer makes of any larger one, must not make the backward plan search for a share
+    # size of that many blocks (267 ms a call at 128 k tokens); the workspace is that of a window as long as the sequence.
+    library = lib.library()
+
+    def workspace(left):
+        p = problem(seqlen, seqlen, left, 0, batch=2, heads_q=16, heads_kv=4)
+        return library.b200fa_sink_bwd_workspace_bytes(ctypes.byref(p), 4)
+
+    start = time.perf_counter()
+    for _ in range(20):
+        size = workspace(2**30)
+    assert time.perf_counter() - start < 0.5  # 20 plans: 0.7 to 5 s with the search, below a millisecond without
+    assert size == workspace(seqlen)

@@ -919,6 +919,8 @@ static int sink_share_rows(const b200fa_problem& p, int sink) {
   const int64_t average = p.heads_kv * row_blocks * (window_blocks + ceil_div(sink, kBlockN)) / 148;
   int64_t blocks = window_blocks > 4 ? window_blocks : 4;
   if (blocks < average / 8) blocks = average / 8;
+  // Here, because the search below takes as many steps: a bound of 2^30 keys, meant as none, took it up to 267 ms a call.
+  if (blocks * 2 * kBlockM > (int64_t)p.seqlen_q) return 0;  // (packed: no sequence can have two shares)
   if (!packed) {
     // One CTA runs per SM, so a launch of two or three waves ends with a full or an almost empty one depending on the number
     // of shares: take the size, up to twice the smallest, with the least product of waves and largest CTA (2 x 4096 tokens,
@@ -932,8 +934,8 @@ static int sink_share_rows(const b200fa_problem& p, int sink) {
       if (best == 0 || cost < best_cost) best = size, best_cost = cost;
     }
     blocks = best;
+    if (blocks * 2 * kBlockM > (int64_t)p.seqlen_q) return 0;
   }
-  if (blocks * 2 * kBlockM > (int64_t)p.seqlen_q) return 0;  // (packed: no sequence can have two shares)
   return (int)(blocks * kBlockM);
 }
 
