@@ -144,3 +144,18 @@ def test_plan_of_a_window_wider_than_any_sequence_is_quick(seqlen):
         size = workspace(2**30)
     assert time.perf_counter() - start < 0.5  # 20 plans: 0.7 to 5 s with the search, below a millisecond without
     assert size == workspace(seqlen)
+
+
+def test_forward_mode_derivatives_are_refused_not_dropped():
+    q = torch.randn(1, 8, 2, 64, dtype=torch.bfloat16)
+    cache = torch.randn(4, 16, 2, 64, dtype=torch.bfloat16)
+    table, lengths = torch.zeros(1, 4, dtype=torch.int32), torch.ones(1, dtype=torch.int32)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(q, torch.ones_like(q))
+        for arguments in ((dual, q, q), (q, dual, q), (q, q, dual)):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                zigfa.flash_attn_sink_func(*arguments, 2, causal=True, window_size=(3, 0))
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            zigfa.flash_attn_paged_func(dual[:, 0], cache, cache, table, lengths)
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            zigfa.append_paged_kv(dual, q, cache, cache, table, lengths)

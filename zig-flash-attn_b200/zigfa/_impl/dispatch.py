@@ -12,6 +12,7 @@ import functools
 import struct
 
 import torch
+from torch.autograd import forward_ad
 
 from . import lib as _lib
 
@@ -77,7 +78,14 @@ def readable(tensor):
     return tensor.clone(memory_format=torch.contiguous_format)
 
 
+def refuse_tangents(what, *tensors):
+    """Forward-mode derivatives: a call that does not go through an autograd Function would drop them silently."""
+    if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(tensor).tangent is not None for tensor in tensors):
+        raise NotImplementedError(f"{what} has no forward-mode derivative")
+
+
 def refuse_gradients(what, *tensors):
+    refuse_tangents(what, *tensors)
     if torch.is_grad_enabled():
         for tensor in tensors:
             if tensor.requires_grad:

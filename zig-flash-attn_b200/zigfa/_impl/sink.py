@@ -10,7 +10,7 @@ import torch
 
 from . import lib as _lib
 from . import ops
-from .dispatch import PACK_BWD, PACK_FWD, define, entry, on_device, readable, stream_of
+from .dispatch import PACK_BWD, PACK_FWD, define, entry, on_device, readable, refuse_tangents, stream_of
 
 BF16, INT32 = torch.bfloat16, torch.int32
 
@@ -158,6 +158,7 @@ def flash_attn_sink(q, k, v, cu_seqlens_q, cu_seqlens_k, sink_size, softmax_scal
     ops.check_sink_size(sink_size)
     left, right = window_size
     ops.require_window(left, right)
+    refuse_tangents("attention with sinks", q, k, v)
     softmax_scale = ops.default_softmax_scale(softmax_scale, q.shape[-1])
     if not softmax_scale > 0:
         raise ValueError(f"attention with sinks needs a positive softmax_scale, got {softmax_scale}")
