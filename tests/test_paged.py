@@ -227,3 +227,49 @@ def test_packed_arguments_have_the_layout_of_the_structures():
                     yield item
 
         assert list(read(filled)) == list(range(1, len(kinds) + 1)), name
+
+
+def test_writing_into_a_cache_is_seen_by_autograd():
+    """A backward pass that has saved a cache must not read what was written into it afterwards."""
+    def fill(*caches):
+        for tensor in caches:
+            tensor.data.fill_(7)  # as a kernel does, without telling autograd
+
+    with torch.library._scoped_library("zigfa", "IMPL") as stand_in:  # CPU kernels in the operators' place, for this test
+        stand_in.impl("append_kv", lambda k, v, k_cache, v_cache, *unused: fill(k_cache, v_cache), "CPU")
+        stand_in.impl("copy_pages", lambda k_cache, v_cache, *unused: fill(k_cache, v_cache), "CPU")
+        rows, table, lengths = torch.ones(1, 1, 2, 64, dtype=torch.bfloat16), ints(1, 4), ints(1)
+        for write in (lambda k, v: zigfa.append_paged_kv(rows, rows, k, v, table, lengths),
+                      lambda k, v: zigfa.copy_kv_pages(k, v, ints(1), ints(1))):
+            for saved in (0, 1):
+                caches = [cache(), cache()]
+                weight = torch.ones(1, requires_grad=True)
+                product = (weight * caches[saved]).sum()
+                write(*caches)
+                assert (caches[saved] == 7).all()
+                with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                    product.backward()
+            with torch.inference_mode():
+                write(cache(), cache())
+
+
+def test_the_short_way_counts_the_versions_too(monkeypatch):
+    """The same for plain CUDA tensors, which do not pass through the dispatcher; here with the launch left out."""
+    from zigfa._impl import dispatch
+
+    calls = []
+    schema = "version_probe(Tensor x, Tensor(a!) y) -> ()"
+    probe = dispatch.define(schema, lambda x, y: calls.append(1) and None, lambda *unused: None, written=((1, "y"),))
+
+    class Plain(torch.Tensor):
+        is_cuda = True
+
+    monkeypatch.setattr(dispatch, "_PLAIN", (Plain, torch.Tensor))
+    x, y = torch.zeros(3).as_subclass(Plain), torch.zeros(3)
+    before = y._version
+    probe(x, y)
+    assert calls == [1] and y._version == before + 1 and x._version == 0
+    with torch.inference_mode():
+        frozen = torch.zeros(3)
+        probe(torch.zeros(3).as_subclass(Plain), frozen)
+    assert calls == [1, 1]

@@ -470,3 +470,24 @@ def test_ops_pass_the_library_checks_and_compile():
         got = torch.compile(step, fullgraph=True)(q, k, *caches[1], table, lengths, refs)
     torch._dynamo.reset()
     assert all(torch.equal(a, b) for a, b in zip(want, got)) and all(torch.equal(a, b) for a, b in zip(*caches))
+
+
+def test_writes_raise_the_version_of_the_caches():
+    torch.manual_seed(15)
+    table, held, rows = ints([[0, 1]]), ints([3]), randn(1, 1, 2, 64)
+    writes = (lambda k, v: zigfa.append_paged_kv(rows, rows, k, v, table, held), lambda k, v: zigfa.copy_kv_pages(k, v, ints([0]), ints([2])),
+              lambda k, v: torch.ops.zigfa.append_kv(rows, rows, k, v, table, held, None),
+              lambda k, v: torch.ops.zigfa.copy_pages(k, v, ints([0]), ints([2])))
+    for write in writes:
+        k, v = randn(4, 16, 2, 64), randn(4, 16, 2, 64)
+        before = k._version, v._version
+        write(k, v)
+        assert k._version > before[0] and v._version > before[1]
+        # training over a cached prefix: the attention has saved views of the cache
+        q = randn(1, 32, 2, 64).requires_grad_()
+        out = zigfa.flash_attn_func(q, k[:2].reshape(1, 32, 2, 64), v[:2].reshape(1, 32, 2, 64), causal=True)
+        write(k, v)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            out.sum().backward()
+        with torch.inference_mode():
+            write(randn(4, 16, 2, 64), randn(4, 16, 2, 64))

@@ -13,6 +13,7 @@ import struct
 
 import torch
 from torch.autograd import forward_ad
+from torch.autograd.graph import increment_version
 
 from . import lib as _lib
 
@@ -31,19 +32,30 @@ PACK_APPEND = struct.Struct(f"@{KV_CACHE}2P6qq3Pq2i").pack
 PACK_PAGES = struct.Struct("@5iPq7PN").pack
 
 
-def define(schema, implementation, fake):
-    """Registers zigfa::<schema> and returns the function that the host layer calls."""
+def define(schema, implementation, fake, written=()):
+    """Registers zigfa::<schema> and returns the function that the host layer calls. `written` = (position, name) of the
+    arguments that the operator writes into: their version counters go up, as with any in-place operation, so that a
+    backward pass that has saved one of them raises instead of reading the new values."""
     name = schema.split("(")[0]
-    _library.define(schema)
-    _library.impl(name, implementation, "CUDA")
-    torch.library.register_fake(f"zigfa::{name}", fake, lib=_library)
+    if written:  # as the other operators that write into their arguments: the registration counts the versions
+        op = torch.library.custom_op(f"zigfa::{name}", implementation, mutates_args=[argument for _, argument in written],
+                                     device_types="cuda", schema=schema[len(name):])
+        op.register_fake(fake)
+    else:
+        _library.define(schema)
+        _library.impl(name, implementation, "CUDA")
+        torch.library.register_fake(f"zigfa::{name}", fake, lib=_library)
     op = getattr(torch.ops.zigfa, name).default
 
     @functools.wraps(implementation)
     def call(*arguments):
         first = arguments[0]
         if type(first) in _PLAIN and first.is_cuda and not _is_compiling() and not _modes():
-            return implementation(*arguments)
+            result = implementation(*arguments)
+            for position, _ in written:
+                if not arguments[position].is_inference():  # those have no version counter
+                    increment_version(arguments[position])
+            return result
         return op(*arguments)  # traced, transformed, or without a kernel for the device
 
     return call

@@ -208,6 +208,7 @@ append_kv = define(
     "Tensor? cu_seqlens) -> ()",
     _append_kv,
     lambda *unused: None,
+    written=((2, "k_cache"), (3, "v_cache")),
 )
 
 
@@ -229,6 +230,7 @@ copy_pages = define(
     "copy_pages(Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor source_pages, Tensor target_pages) -> ()",
     _copy_pages,
     lambda *unused: None,
+    written=((0, "k_cache"), (1, "v_cache")),
 )
 
 
