@@ -171,7 +171,7 @@ int b200fa_query_blocks_host(const b200fa_problem* problem, int32_t seq, int32_t
 /* ---- Sliding window with sinks (no counterpart in the reference): b200fa_fwd and b200fa_bwd with the first sink_size
  * keys of every sequence visible to each query row that the right bound lets see them, in front of the window. Without a
  * left bound sink_size has no effect. Not for inter-sequence batches; softmax_scale > 0. In a packed batch, what
- * stands in rows behind the last sequence, NaN included, has no effect on any result. */
+ * stands in rows behind the last sequence, NaN included, has no effect on any result, whatever the window and sink_size. */
 size_t b200fa_sink_fwd_workspace_bytes(const b200fa_problem* problem, int32_t sink_size);
 int b200fa_sink_fwd(const b200fa_fwd_args* args, int32_t sink_size, void* stream);
 size_t b200fa_sink_bwd_workspace_bytes(const b200fa_problem* problem, int32_t sink_size);

@@ -253,3 +253,27 @@ def test_two_streams_at_once():
     torch.cuda.synchronize()
     for i, out in enumerate(got):
         assert torch.equal(out, want[i % 2])
+
+
+@pytest.mark.parametrize("left, right, sink", [(100, 0, 0), (-1, 0, 4), (-1, -1, 0), (-1, 30, 200), (0, -1, 0)])
+@pytest.mark.parametrize("heads, d", [((4, 4), 128), ((8, 2), 64), ((3, 1), 96), ((4, 2), 256), ((2, 1), 512)])
+def test_packed_batches_without_sinks_or_a_left_bound_do_not_see_what_stands_behind_them(left, right, sink, heads, d):
+    """The promise about rows behind the last sequence holds whatever the window and the sinks are."""
+    torch.manual_seed(d + left + sink)
+    lengths_q, lengths_k, padding = (300, 0, 77, 129), (300, 5, 200, 130), 70
+    total_q, total_k = sum(lengths_q), sum(lengths_k)
+    cu_q, cu_k = (ints([0, *torch.tensor(x).cumsum(0).tolist()]) for x in (lengths_q, lengths_k))
+    q, k, v, dout = (randn(total + padding, h, d) for total, h in ((total_q, heads[0]), (total_k, heads[1]), (total_k, heads[1]), (total_q, heads[0])))
+    for x, total in ((q, total_q), (k, total_k), (v, total_k), (dout, total_q)):
+        x[total:] = float("nan")
+    leaves = [x.requires_grad_(d < 512) for x in (q, k, v)]
+    out, lse = zigfa.flash_attn_varlen_sink_func(*leaves, cu_q, cu_k, 300, 300, sink, window_size=(left, right), return_attn_probs=True)
+    got = dict(zip(("dq", "dk", "dv"), torch.autograd.grad(out, leaves, dout) if d < 512 else ()), out=out.detach())
+    row_q = row_k = 0
+    for lq, lk in zip(lengths_q, lengths_k):
+        rows, keys = slice(row_q, row_q + lq), slice(row_k, row_k + lk)
+        want = plain.with_tolerances(q[rows].detach(), k[keys].detach(), v[keys].detach(), dout[rows] if d < 512 else None, plain.visible(lq, lk, left, right, sink), d**-0.5)
+        plain.assert_within("lse", lse[:, rows], *want.pop("lse"), (heads, lq, lk))
+        for name, (value, tolerance) in want.items():
+            plain.assert_within(name, got[name][keys if name in ("dk", "dv") else rows], value, tolerance, (heads, d, lq, lk))
+        row_q, row_k = row_q + lq, row_k + lk

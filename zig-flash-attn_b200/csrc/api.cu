@@ -147,14 +147,17 @@ static int validate_problem(const b200fa_problem& p) {
   return B200FA_OK;
 }
 
-// Sinks matter in front of a window only: without a left bound every key is visible anyway.
-static int sinks_of(const b200fa_problem& p, int sink_size) { return p.window_left < 0 ? 0 : sink_size; }
+// Sinks matter in front of a window only: without a left bound every key is visible anyway. Fixed-length problems without
+// them take the plain instances; packed ones do not, because of what may stand behind their sequences.
+static int sinks_of(const b200fa_problem& p, int sink_size) {
+  const int sinks = p.window_left < 0 ? 0 : sink_size;
+  return sinks > 0 || (p.cu_seqlens_q && !p.visibility_bits) ? sinks : kNoSinks;
+}
 
 static int validate_sinks(const b200fa_problem& p, int sink_size) {
-  B200FA_REQUIRE(sink_size >= 0, "sink_size must not be negative");
   B200FA_REQUIRE(sink_size == 0 || !p.visibility_bits, "inter-sequence attention has no sinks");
   // masked scores are -inf before they are scaled
-  B200FA_REQUIRE(sinks_of(p, sink_size) == 0 || p.softmax_scale > 0.f, "attention with sinks needs a positive softmax_scale");
+  B200FA_REQUIRE(sinks_of(p, sink_size) < 0 || p.softmax_scale > 0.f, "attention with sinks needs a positive softmax_scale");
   return B200FA_OK;
 }
 
@@ -200,16 +203,15 @@ size_t b200fa_sink_fwd_workspace_bytes(const b200fa_problem* p, int32_t sink_siz
   return static_cast<size_t>(work_list_entries(p->seqlen_q, p->batch, tile_rows)) * 8;
 }
 
-int b200fa_fwd(const b200fa_fwd_args* args, void* stream) { return b200fa_sink_fwd(args, 0, stream); }
-
-int b200fa_sink_fwd(const b200fa_fwd_args* args, int32_t sink_size, void* stream) {
+// `sink_size` = kNoSinks: plain attention.
+static int run_fwd(const b200fa_fwd_args* args, int sink_size, void* stream) {
   if (!args) {
     set_error("null arguments");
     return B200FA_ERR_INVALID;
   }
   const b200fa_problem& p = args->problem;
   int status = validate_problem(p);
-  if (status == B200FA_OK) status = validate_sinks(p, sink_size);
+  if (status == B200FA_OK && sink_size != kNoSinks) status = validate_sinks(p, sink_size);
   if (status != B200FA_OK) return status;
   B200FA_REQUIRE(strides_ok(args->q_stride) && strides_ok(args->k_stride) && strides_ok(args->v_stride) &&
                      strides_ok(args->out_stride),
@@ -218,7 +220,14 @@ int b200fa_sink_fwd(const b200fa_fwd_args* args, int32_t sink_size, void* stream
   if (p.batch == 0 || p.seqlen_q == 0) return B200FA_OK;
   B200FA_REQUIRE(args->q && args->out && args->softmax_lse, "null tensor pointer");
   B200FA_REQUIRE(p.seqlen_k == 0 || (args->k && args->v), "null tensor pointer");
-  return launch_fwd(*args, sinks_of(p, sink_size), static_cast<cudaStream_t>(stream));
+  return launch_fwd(*args, sink_size == kNoSinks ? kNoSinks : sinks_of(p, sink_size), static_cast<cudaStream_t>(stream));
+}
+
+int b200fa_fwd(const b200fa_fwd_args* args, void* stream) { return run_fwd(args, kNoSinks, stream); }
+
+int b200fa_sink_fwd(const b200fa_fwd_args* args, int32_t sink_size, void* stream) {
+  B200FA_REQUIRE(sink_size >= 0, "sink_size must not be negative");
+  return run_fwd(args, sink_size, stream);
 }
 
 int b200fa_set_trace(void* counters) {
@@ -236,22 +245,20 @@ int b200fa_bwd_timing_events(void* const* events) {
   return B200FA_OK;
 }
 
-size_t b200fa_bwd_workspace_bytes(const b200fa_problem* p) { return bwd_workspace_bytes(*p, 0); }
+size_t b200fa_bwd_workspace_bytes(const b200fa_problem* p) { return bwd_workspace_bytes(*p, kNoSinks); }
 
 size_t b200fa_sink_bwd_workspace_bytes(const b200fa_problem* p, int32_t sink_size) {
   return bwd_workspace_bytes(*p, sinks_of(*p, sink_size));
 }
 
-int b200fa_bwd(const b200fa_bwd_args* args, void* stream) { return b200fa_sink_bwd(args, 0, stream); }
-
-int b200fa_sink_bwd(const b200fa_bwd_args* args, int32_t sink_size, void* stream) {
+static int run_bwd(const b200fa_bwd_args* args, int sink_size, void* stream) {
   if (!args) {
     set_error("null arguments");
     return B200FA_ERR_INVALID;
   }
   const b200fa_problem& p = args->problem;
   int status = validate_problem(p);
-  if (status == B200FA_OK) status = validate_sinks(p, sink_size);
+  if (status == B200FA_OK && sink_size != kNoSinks) status = validate_sinks(p, sink_size);
   if (status != B200FA_OK) return status;
   B200FA_REQUIRE(strides_ok(args->q_stride) && strides_ok(args->k_stride) && strides_ok(args->v_stride) &&
                      strides_ok(args->out_stride) && strides_ok(args->dout_stride) && strides_ok(args->dq_stride) &&
@@ -269,7 +276,14 @@ int b200fa_sink_bwd(const b200fa_bwd_args* args, int32_t sink_size, void* stream
   for (const void* pointer : aligned16)
     B200FA_REQUIRE(reinterpret_cast<uintptr_t>(pointer) % 16 == 0, "tensor pointers must be 16-byte aligned");
   B200FA_REQUIRE(reinterpret_cast<uintptr_t>(args->softmax_lse) % 4 == 0, "softmax_lse must be 4-byte aligned");
-  return launch_bwd(*args, sinks_of(p, sink_size), static_cast<cudaStream_t>(stream));
+  return launch_bwd(*args, sink_size == kNoSinks ? kNoSinks : sinks_of(p, sink_size), static_cast<cudaStream_t>(stream));
+}
+
+int b200fa_bwd(const b200fa_bwd_args* args, void* stream) { return run_bwd(args, kNoSinks, stream); }
+
+int b200fa_sink_bwd(const b200fa_bwd_args* args, int32_t sink_size, void* stream) {
+  B200FA_REQUIRE(sink_size >= 0, "sink_size must not be negative");
+  return run_bwd(args, sink_size, stream);
 }
 
 }  // extern "C"

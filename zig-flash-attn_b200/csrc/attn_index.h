@@ -90,6 +90,10 @@ B200FA_HD void sink_query_block_range(Band band, int lq, int c0, int c1, int sin
   band_query_block_range(band, lq, c0, c1, first, last);
 }
 
+// Sinks of a launch of the instances without them. (Packed batches of the sink entries take the kSink instances with 0 sinks
+// too: only these keep rows behind the end of a sequence out of the products.)
+constexpr int kNoSinks = -1;
+
 // Problem description common to forward and backward kernels (plain data; passed by value to kernels).
 struct Problem {
   int batch;        // batch entries (fixed length) or sequences (varlen / inter-sequence)
@@ -104,7 +108,7 @@ struct Problem {
   const int32_t* bits_t;        // transpose
   const int32_t* window_sizes;  // (2, n) or null
   int words;
-  int sink;                     // the first `sink` keys stay visible in front of the window (instances with kSink)
+  int sink;                     // the first `sink` keys stay visible in front of the window; kNoSinks: instances without kSink
 };
 
 struct SeqInfo {

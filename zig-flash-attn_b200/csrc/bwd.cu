@@ -1020,7 +1020,7 @@ static int launch_main(const b200fa_bwd_args& a, const BwdParams& p, dim3 grid, 
     return B200FA_OK;
   };
   static bool set_plain[64] = {false}, set_pivot[64] = {false}, set_sink[64] = {false}, set_sink_pivot[64] = {false};
-  if (p.prob.sink > 0) {
+  if (p.prob.sink >= 0) {
     status = p.pivot_key ? launch(&bwd_kernel<D, true, true>, set_sink_pivot) : launch(&bwd_kernel<D, false, true>, set_sink);
   } else {
     status = p.pivot_key ? launch(&bwd_kernel<D, true, false>, set_pivot) : launch(&bwd_kernel<D, false, false>, set_plain);

@@ -604,7 +604,7 @@ int launch_bwd_main_d256(const b200fa_bwd_args& a, const BwdParams& p, dim3 grid
     const char* setting = std::getenv("B200FA_BWD_D256_PAIR");
     return setting != nullptr && setting[0] == '1';
   }();
-  if (paired && !p.pivot_key && p.prob.sink == 0) return launch_bwd_main_d256_pair(a, p, grid, dq_accum, stat_rows, stream);
+  if (paired && !p.pivot_key && p.prob.sink < 0) return launch_bwd_main_d256_pair(a, p, grid, dq_accum, stat_rows, stream);
   const b200fa_problem& bp = a.problem;
   const bool packed = bp.cu_seqlens_q != nullptr;
   const int64_t rows_q = bp.seqlen_q, rows_k = bp.seqlen_k;
@@ -646,7 +646,7 @@ int launch_bwd_main_d256(const b200fa_bwd_args& a, const BwdParams& p, dim3 grid
     return B200FA_OK;
   };
   static bool set_plain[64] = {false}, set_pivot[64] = {false}, set_sink[64] = {false}, set_sink_pivot[64] = {false};
-  if (p.prob.sink > 0) {
+  if (p.prob.sink >= 0) {
     status = p.pivot_key ? launch(&bwd_d256_kernel<true, true>, set_sink_pivot) : launch(&bwd_d256_kernel<false, true>, set_sink);
   } else {  // pivot gradients on request (b200fa_set_pivot_ds)
     status = p.pivot_key ? launch(&bwd_d256_kernel<true, false>, set_pivot) : launch(&bwd_d256_kernel<false, false>, set_plain);

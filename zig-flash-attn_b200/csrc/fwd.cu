@@ -706,7 +706,7 @@ static SplitPlan plan_split(const b200fa_problem& bp, int sink) {
   const int64_t tiles = (int64_t)bp.batch * (bp.heads_q >> pack_shift_of(bp)) * ceil_div(bp.seqlen_q, tile_tokens);
   int64_t keys = bp.seqlen_k;
   if (bp.window_left >= 0) {
-    const int64_t reach = (int64_t)bp.window_left + imin(bp.seqlen_q, tile_tokens) + imax(bp.window_right, 0) + sink;
+    const int64_t reach = (int64_t)bp.window_left + imin(bp.seqlen_q, tile_tokens) + imax(bp.window_right, 0) + imax(sink, 0);
     keys = keys < reach ? keys : reach;
   }
   const int64_t blocks = (keys + kBlockN - 1) / kBlockN;
@@ -898,7 +898,7 @@ static int launch_fwd_d(const b200fa_fwd_args& a, int sink, cudaStream_t stream)
   }
   const int grid = p.num_tiles < sms ? p.num_tiles : sms;
   // Instances: split-KV, problems with visibility bits (inter-sequence batches), the plain one, and the first and the
-  // last of these with sinks.
+  // last of these for the sink entries (sink >= 0).
   auto launch = [&](auto kernel, bool (&attribute_set)[64]) -> int {
     const int set = set_dynamic_smem_once(reinterpret_cast<const void*>(kernel), Cfg::kSmemBytes, attribute_set);
     if (set != B200FA_OK) return set;
@@ -907,7 +907,7 @@ static int launch_fwd_d(const b200fa_fwd_args& a, int sink, cudaStream_t stream)
   };
   static bool set_split[64] = {false}, set_bits[64] = {false}, set_plain[64] = {false};
   static bool set_sink_split[64] = {false}, set_sink[64] = {false};
-  if (sink > 0) {
+  if (sink >= 0) {
     status = split ? launch(&fwd_kernel<D, true, false, true>, set_sink_split)
                    : launch(&fwd_kernel<D, false, false, true>, set_sink);
   } else if (split) {
@@ -945,7 +945,7 @@ int launch_fwd(const b200fa_fwd_args& a, int sink, cudaStream_t stream) {
         const char* value = getenv("B200FA_FWD_D256_PAIR");
         return value && value[0] == '1';
       }();
-      return pair_kernel && sink == 0 ? launch_fwd_256_pair(a, stream) : launch_fwd_256(a, sink, stream);
+      return pair_kernel && sink < 0 ? launch_fwd_256_pair(a, stream) : launch_fwd_256(a, sink, stream);
     }
     case 512:
       return launch_fwd_512(a, sink, stream);

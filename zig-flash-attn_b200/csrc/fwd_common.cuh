@@ -283,7 +283,7 @@ int prepare_forward(const b200fa_fwd_args& a, cudaStream_t stream, int head_dim,
                     FwdParams* p, CUtensorMap* map_q, CUtensorMap* map_k, CUtensorMap* map_v, bool* nothing_to_do,
                     int v_box_rows = 0 /* rows per TMA box of V when they differ from those of K */,
                     int pack_shift = 0 /* log2 of the query heads packed into the rows of a work item */,
-                    int sink = 0 /* first keys that stay visible in front of the window (instances with kSink) */);
+                    int sink = kNoSinks /* first keys that stay visible in front of the window (instances with kSink) */);
 // A zeroed work-item counter for one launch on `stream`: the next slot of the device's ring of 4096 counters inside the
 // library, reset by a memset node ahead of the kernel. Launches share a slot only 4096 launches apart (or through a
 // captured graph, which keeps its slot); see the contract at its definition in fwd.cu.

@@ -475,7 +475,7 @@ int launch_fwd_256(const b200fa_fwd_args& a, int sink, cudaStream_t stream) {
   };
   static bool set_bits[64] = {false}, set_plain[64] = {false}, set_sink[64] = {false};
   status = a.problem.visibility_bits ? launch(&fwd_d256_kernel<true, false>, set_bits)
-           : sink > 0                ? launch(&fwd_d256_kernel<false, true>, set_sink)
+           : sink >= 0               ? launch(&fwd_d256_kernel<false, true>, set_sink)
                                      : launch(&fwd_d256_kernel<false, false>, set_plain);
   if (status != B200FA_OK) return status;
   B200FA_CUDA_CHECK(cudaGetLastError());

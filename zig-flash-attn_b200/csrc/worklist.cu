@@ -178,7 +178,7 @@ Problem to_problem(const b200fa_problem& in) {
   p.bits_t = in.visibility_bits_t;
   p.window_sizes = in.window_sizes;
   p.words = (in.batch + 31) / 32;
-  p.sink = 0;
+  p.sink = kNoSinks;
   return p;
 }
 

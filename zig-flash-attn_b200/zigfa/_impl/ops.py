@@ -151,7 +151,12 @@ def launch_forward(q, k, v, out, softmax_lse, cu_seqlens_q, cu_seqlens_k, softma
     library = _lib.library()
     problem = _lib.make_problem(q, k, cu_seqlens_q, cu_seqlens_k, softmax_scale, left, right, *(interseq or ()))
     with torch.cuda.device(q.device):
-        workspace = _workspace(library.b200fa_sink_fwd_workspace_bytes(ctypes.byref(problem), sink), q.device)
+        workspace = _workspace(
+            library.b200fa_sink_fwd_workspace_bytes(ctypes.byref(problem), sink)
+            if sink
+            else library.b200fa_fwd_workspace_bytes(ctypes.byref(problem)),
+            q.device,
+        )
         args = _lib.FwdArgs(
             problem=problem,
             q=q.data_ptr(),
@@ -167,7 +172,10 @@ def launch_forward(q, k, v, out, softmax_lse, cu_seqlens_q, cu_seqlens_k, softma
             workspace=workspace.data_ptr(),
             workspace_bytes=workspace.numel(),
         )
-        _lib.check(library.b200fa_sink_fwd(ctypes.byref(args), sink, _stream(q.device)))
+        if sink:
+            _lib.check(library.b200fa_sink_fwd(ctypes.byref(args), sink, _stream(q.device)))
+        else:
+            _lib.check(library.b200fa_fwd(ctypes.byref(args), _stream(q.device)))
 
 
 def launch_backward(
@@ -178,7 +186,12 @@ def launch_backward(
     library = _lib.library()
     problem = _lib.make_problem(q, k, cu_seqlens_q, cu_seqlens_k, softmax_scale, left, right, *(interseq or ()))
     with torch.cuda.device(q.device):
-        workspace = _workspace(library.b200fa_sink_bwd_workspace_bytes(ctypes.byref(problem), sink), q.device)
+        workspace = _workspace(
+            library.b200fa_sink_bwd_workspace_bytes(ctypes.byref(problem), sink)
+            if sink
+            else library.b200fa_bwd_workspace_bytes(ctypes.byref(problem)),
+            q.device,
+        )
         strides = {
             name + "_stride": _lib.strides3(tensor, packed)
             for name, tensor in dict(q=q, k=k, v=v, out=out, dout=dout, dq=dq, dk=dk, dv=dv).items()
@@ -199,7 +212,10 @@ def launch_backward(
             workspace_bytes=workspace.numel(),
             **strides,
         )
-        _lib.check(library.b200fa_sink_bwd(ctypes.byref(args), sink, _stream(q.device)))
+        if sink:
+            _lib.check(library.b200fa_sink_bwd(ctypes.byref(args), sink, _stream(q.device)))
+        else:
+            _lib.check(library.b200fa_bwd(ctypes.byref(args), _stream(q.device)))
 
 
 def forward_impl(q, k, v, cu_seqlens_q, cu_seqlens_k, softmax_scale, left, right, interseq=None, direction=FORWARD, sink=0):
