@@ -176,6 +176,11 @@ size_t b200fa_sink_fwd_workspace_bytes(const b200fa_problem* problem, int32_t si
 int b200fa_sink_fwd(const b200fa_fwd_args* args, int32_t sink_size, void* stream);
 size_t b200fa_sink_bwd_workspace_bytes(const b200fa_problem* problem, int32_t sink_size);
 int b200fa_sink_bwd(const b200fa_bwd_args* args, int32_t sink_size, void* stream);
+/* The same for contiguous results (out and softmax_lse; dq, dk and dv): the rows of a packed batch that belong to no sequence,
+ * in front of cu_seqlens[0] and at or behind cu_seqlens[batch], which the calls above leave as they are, are filled with
+ * zeros, -inf in softmax_lse. */
+int b200fa_sink_fwd_all_rows(const b200fa_fwd_args* args, int32_t sink_size, void* stream);
+int b200fa_sink_bwd_all_rows(const b200fa_bwd_args* args, int32_t sink_size, void* stream);
 /* b200fa_key_blocks_host and b200fa_query_blocks_host with sinks. */
 int b200fa_sink_key_blocks_host(const b200fa_problem* problem, int32_t sink_size, int32_t seq, int32_t m0, int32_t m1,
                                 int32_t* out, int32_t max_blocks);

@@ -159,3 +159,27 @@ def test_forward_mode_derivatives_are_refused_not_dropped():
             zigfa.flash_attn_paged_func(dual[:, 0], cache, cache, table, lengths)
         with pytest.raises(NotImplementedError, match="forward-mode"):
             zigfa.append_paged_kv(dual, q, cache, cache, table, lengths)
+
+
+def test_entries_that_fill_all_rows_want_contiguous_results():
+    library = lib.library()
+    aligned = 1 << 20  # passes the alignment checks; nothing dereferences it on these paths
+    packed = problem(64, 64, 10, 0, batch=0, cu_seqlens_q=aligned, cu_seqlens_k=aligned)
+    row, heads = lib.Stride3(0, 4 * 128, 128), lib.Stride3(0, 2 * 128, 128)
+    good = dict(problem=packed, out=aligned, softmax_lse=aligned, out_stride=row, lse_stride=lib.Stride2(0, 64))
+    for changes, message in [(dict(out_stride=lib.Stride3(0, 8 * 128, 128)), "contiguous"), (dict(out_stride=lib.Stride3(0, 4 * 128, 256)), "contiguous"),
+                             (dict(lse_stride=lib.Stride2(0, 72)), "contiguous"), (dict(out=None), "pointer"), (dict(out=aligned + 8), "aligned"),
+                             (dict(softmax_lse=None), "null")]:
+        assert library.b200fa_sink_fwd_all_rows(ctypes.byref(lib.FwdArgs(**{**good, **changes})), 4, None) == -1, changes
+        assert message in lib.last_error(), changes
+    good = dict(problem=packed, dq=aligned, dk=aligned, dv=aligned, dq_stride=row, dk_stride=heads, dv_stride=heads)
+    for changes, message in [(dict(dq_stride=heads), "contiguous"), (dict(dv_stride=row), "contiguous"), (dict(dk=None), "pointer"),
+                             (dict(dv=aligned + 4), "aligned")]:
+        assert library.b200fa_sink_bwd_all_rows(ctypes.byref(lib.BwdArgs(**{**good, **changes})), 4, None) == -1, changes
+        assert message in lib.last_error(), changes
+    for function in (library.b200fa_sink_fwd_all_rows, library.b200fa_sink_bwd_all_rows):
+        assert function(None, 4, None) == -1
+    empty = problem(0, 0, 10, 0, batch=0, cu_seqlens_q=aligned, cu_seqlens_k=aligned)
+    assert library.b200fa_sink_fwd_all_rows(ctypes.byref(lib.FwdArgs(problem=empty, out_stride=row)), 4, None) == 0  # no rows, no launch
+    fixed = lib.FwdArgs(problem=problem(0, 0, 10, 0, batch=0))  # nothing stands between the sequences of a fixed-length batch
+    assert library.b200fa_sink_fwd_all_rows(ctypes.byref(fixed), 4, None) == 0

@@ -277,3 +277,28 @@ def test_packed_batches_without_sinks_or_a_left_bound_do_not_see_what_stands_beh
         for name, (value, tolerance) in want.items():
             plain.assert_within(name, got[name][keys if name in ("dk", "dv") else rows], value, tolerance, (heads, d, lq, lk))
         row_q, row_k = row_q + lq, row_k + lk
+
+
+@pytest.mark.parametrize("d", [64, 72, 128, 256, 512])
+@pytest.mark.parametrize("window, sink", [((50, 0), 4), ((50, 0), 0), ((-1, 0), 0)])
+def test_rows_of_no_sequence_come_out_as_zeros(d, window, sink):
+    """What the functions return for rows in front of the first and behind the last sequence is defined: zeros, a log-sum-exp
+    of -inf, and gradients of zero, so that a layer in front may sum over all rows."""
+    torch.manual_seed(d)
+    for cu_q, cu_k, total_q, total_k in (([0, 150, 400], [0, 20, 300], 1000, 333), ([3, 100], [40, 200], 101, 900), ([0, 64], [0, 64], 64, 64),
+                                         ([7], [9], 50, 60), ([0, 0], [0, 30], 40, 30), ([0, 5, 5], [0, 0, 0], 6, 3)):
+        leftover = [torch.full((n,), float("nan"), device="cuda", dtype=torch.bfloat16) for n in (total_q * 4 * d, total_k * 2 * d) * 4]
+        del leftover  # the allocator hands this memory out next
+        q, k, v = (randn(n, h, d, requires_grad=d < 512) for n, h in ((total_q, 4), (total_k, 2), (total_k, 2)))
+        dout = torch.ones(total_q, 4, d, device="cuda", dtype=torch.bfloat16)
+        out, lse = zigfa.flash_attn_varlen_sink_func(q, k, v, ints(cu_q), ints(cu_k), 300, 300, sink, window_size=window, return_attn_probs=True)
+        results = [(out.detach(), cu_q)]
+        if d < 512:
+            results += zip(torch.autograd.grad(out, (q, k, v), dout), (cu_q, cu_k, cu_k))
+        for tensor, cu in results:
+            assert torch.isfinite(tensor).all()
+            assert (tensor[:cu[0]] == 0).all() and (tensor[cu[-1]:] == 0).all()
+            if len(cu) > 1 and cu_q[-1] > cu_q[0] and cu_k[-1] > cu_k[0]:
+                assert (tensor[cu[0]:cu[-1]] != 0).any()
+        assert (lse[:, :cu_q[0]] == float("-inf")).all() and (lse[:, cu_q[-1]:] == float("-inf")).all()
+        assert not torch.isnan(lse).any()

@@ -36,6 +36,8 @@ EXPORTS = (
     "b200fa_sink_fwd",
     "b200fa_sink_bwd_workspace_bytes",
     "b200fa_sink_bwd",
+    "b200fa_sink_fwd_all_rows",
+    "b200fa_sink_bwd_all_rows",
     "b200fa_sink_key_blocks_host",
     "b200fa_sink_query_blocks_host",
     "b200fa_paged_decode_workspace_bytes",
@@ -225,8 +227,9 @@ def library() -> ctypes.CDLL:
     for name, args in (("fwd", FwdArgs), ("bwd", BwdArgs)):
         function = getattr(lib, f"b200fa_sink_{name}_workspace_bytes")
         function.restype, function.argtypes = ctypes.c_size_t, [ctypes.POINTER(Problem), ctypes.c_int32]
-        function = getattr(lib, f"b200fa_sink_{name}")
-        function.restype, function.argtypes = ctypes.c_int, [ctypes.POINTER(args), ctypes.c_int32, ctypes.c_void_p]
+        for entry in (f"b200fa_sink_{name}", f"b200fa_sink_{name}_all_rows"):
+            function = getattr(lib, entry)
+            function.restype, function.argtypes = ctypes.c_int, [ctypes.POINTER(args), ctypes.c_int32, ctypes.c_void_p]
     for name in ("key", "query"):
         function = getattr(lib, f"b200fa_sink_{name}_blocks_host")
         function.restype = ctypes.c_int

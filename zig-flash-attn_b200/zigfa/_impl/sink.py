@@ -82,7 +82,7 @@ def _forward(q, k, v, cu_seqlens_q, cu_seqlens_k, softmax_scale, window_left, wi
         *_strides(k, packed), *_strides(v, packed), *_strides(out, packed), 0 if packed else lse_stride[0], lse_stride[-2],
         workspace.data_ptr() if nbytes else 0, nbytes,
     )
-    on_device(device, entry("b200fa_sink_fwd", ctypes.c_int32, ctypes.c_void_p), arguments, sink_size, stream_of(device))
+    on_device(device, entry("b200fa_sink_fwd_all_rows", ctypes.c_int32, ctypes.c_void_p), arguments, sink_size, stream_of(device))
     return out, softmax_lse
 
 
@@ -123,7 +123,7 @@ def _backward(dout, q, k, v, out, softmax_lse, cu_seqlens_q, cu_seqlens_k, softm
         *_strides(dout, packed), *_strides(dq, packed), *stride_dk, *stride_dk, 0 if packed else lse_stride[0], lse_stride[-2],
         workspace.data_ptr(), nbytes,
     )
-    on_device(device, entry("b200fa_sink_bwd", ctypes.c_int32, ctypes.c_void_p), arguments, sink_size, stream_of(device))
+    on_device(device, entry("b200fa_sink_bwd_all_rows", ctypes.c_int32, ctypes.c_void_p), arguments, sink_size, stream_of(device))
     return dq, dk, dv
 
 

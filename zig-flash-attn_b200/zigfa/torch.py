@@ -134,8 +134,8 @@ def flash_attn_varlen_sink_func(
     deterministic: bool = False, return_attn_probs: bool = False,
 ) -> Tensor | tuple[Tensor, Tensor]:
     """flash_attn_sink_func for packed batches (flash_attn_varlen_func): the first `sink_size` keys of every sequence stay
-    visible to its own rows. Rows behind the last sequence are left as they are, and what they hold (NaN included) has no
-    effect on any result."""
+    visible to its own rows. What rows in front of the first or behind the last sequence hold (NaN included) has no effect on
+    any result; they come out as zeros, with a log-sum-exp of -inf and gradients of zero."""
     from ._impl import sink
 
     return sink.flash_attn_sink(q, k, v, cu_seqlens_q, cu_seqlens_k, sink_size, softmax_scale, causal, window_size, deterministic, return_attn_probs)
