@@ -183,3 +183,23 @@ def test_entries_that_fill_all_rows_want_contiguous_results():
     assert library.b200fa_sink_fwd_all_rows(ctypes.byref(lib.FwdArgs(problem=empty, out_stride=row)), 4, None) == 0  # no rows, no launch
     fixed = lib.FwdArgs(problem=problem(0, 0, 10, 0, batch=0))  # nothing stands between the sequences of a fixed-length batch
     assert library.b200fa_sink_fwd_all_rows(ctypes.byref(fixed), 4, None) == 0
+
+
+@pytest.mark.parametrize("tokens, heads_q, heads_kv, d, left, sink", [
+    (131072, 32, 8, 128, 1023, 4), (131072, 32, 8, 128, 1023, 500), (131072, 16, 8, 256, 1023, 500), (16384, 8, 8, 64, 255, 512),
+    (131072, 8, 8, 128, 255, 17), (65536, 32, 8, 128, 255, 4), (4000, 2, 2, 72, 50, 300), (131072, 1, 1, 64, 100, 4)])
+def test_workspace_of_a_packed_backward_pass_does_not_grow_with_the_number_of_documents(tokens, heads_q, heads_kv, d, left, sink):
+    """The FP32 parts of dK and dV belong to sequences of two shares or more, however many short ones there are; and they are
+    no larger than what the pass keeps anyway (1024 documents in 131072 tokens once took 8 GB of parts next to 3 GB)."""
+    library = lib.library()
+
+    def parts(documents):
+        p = problem(tokens, tokens, left, 0, batch=documents, heads_q=heads_q, heads_kv=heads_kv, head_dim=d, cu_seqlens_q=8, cu_seqlens_k=8)
+        plain = library.b200fa_bwd_workspace_bytes(ctypes.byref(p))
+        return library.b200fa_sink_bwd_workspace_bytes(ctypes.byref(p), sink) - plain, plain
+
+    extra, plain = parts(1)
+    assert 0 <= extra <= 1.5 * plain
+    for documents in (2, 100, 1000, 4096):
+        # the list of shares holds 8 bytes per sequence of more than `least` rows, 512 or more; both lists are aligned to 256
+        assert abs(parts(documents)[0] - extra) <= 8 * (tokens // 512) + 512, documents

@@ -302,3 +302,30 @@ def test_rows_of_no_sequence_come_out_as_zeros(d, window, sink):
                 assert (tensor[cu[0]:cu[-1]] != 0).any()
         assert (lse[:, :cu_q[0]] == float("-inf")).all() and (lse[:, cu_q[-1]:] == float("-inf")).all()
         assert not torch.isnan(lse).any()
+
+
+@pytest.mark.parametrize("heads, d, left, sink", [((4, 2), 64, 100, 4), ((2, 2), 128, 300, 300), ((4, 1), 256, 60, 17), ((3, 1), 72, 0, 500)])
+def test_many_short_documents_next_to_long_ones(heads, d, left, sink):
+    """Documents below, at and above the size of a share (512 query rows here and more) in one packed batch."""
+    torch.manual_seed(d + sink)
+    lengths = [int(n) for n in torch.randint(0, 60, (40,))]
+    for place, length in ((0, 513), (5, 2100), (11, 512), (12, 511), (20, 1025), (30, 1024), (40, 3000), (44, 640), (46, 641)):
+        lengths.insert(place, length)
+    other = [n + (i % 3) * 17 if i % 5 else n // 2 for i, n in enumerate(lengths)]
+    lengths[25] = other[25] = 0
+    other[10], lengths[33] = 0, 0
+    cu_q, cu_k = (ints([0, *torch.tensor(x).cumsum(0).tolist()]) for x in (lengths, other))
+    q, k, v = (randn(sum(x), h, d, requires_grad=True) for x, h in ((lengths, heads[0]), (other, heads[1]), (other, heads[1])))
+    dout = randn(sum(lengths), heads[0], d)
+    out = zigfa.flash_attn_varlen_sink_func(q, k, v, cu_q, cu_k, 3000, 3100, sink, window_size=(left, 0))
+    got = dict(zip(("dq", "dk", "dv"), torch.autograd.grad(out, (q, k, v), dout)), out=out.detach())
+    again = torch.autograd.grad(zigfa.flash_attn_varlen_sink_func(q, k, v, cu_q, cu_k, 3000, 3100, sink, window_size=(left, 0)), (k, v), dout)
+    assert torch.equal(again[0], got["dk"]) and torch.equal(again[1], got["dv"])  # parts are added in order
+    row_q = row_k = 0
+    for lq, lk in zip(lengths, other):
+        rows, keys = slice(row_q, row_q + lq), slice(row_k, row_k + lk)
+        want = plain.with_tolerances(q[rows].detach(), k[keys].detach(), v[keys].detach(), dout[rows], plain.visible(lq, lk, left, 0, sink), d**-0.5)
+        want.pop("lse")
+        for name, (value, tolerance) in want.items():
+            plain.assert_within(name, got[name][keys if name in ("dk", "dv") else rows], value, tolerance, (d, lq, lk))
+        row_q, row_k = row_q + lq, row_k + lk

@@ -762,7 +762,7 @@ struct PivotFix {
 };
 
 // dK and dV of the key blocks whose work was dealt out in shares: the sum of the shares' parts, in their order. A
-// block of 256 threads per (key block of a sequence, key head, 256 / (D / 4) rows), further blocks of the postprocess
+// block of 256 threads per (key block of a sequence, or of an entry of the shares' list where these are fewer, key head, 256 / (D / 4) rows), further blocks of the postprocess
 // launch; a thread adds four columns of dV and of dK.
 template <int D>
 __device__ __forceinline__ void join_sink_shares(const BwdParams& p, int block, int kv_head) {
@@ -770,15 +770,23 @@ __device__ __forceinline__ void join_sink_shares(const BwdParams& p, int block, 
   const Problem& pr = p.prob;
   constexpr int per_block = kBlockN / kRows;
   const int group = block / per_block, r = (block - group * per_block) * kRows + threadIdx.x / kQuads;
-  const int seq = group / p.sinks.blocks, n_block = group - seq * p.sinks.blocks;
+  const int entry = group / p.sinks.blocks, n_block = group - entry * p.sinks.blocks;
+  int seq = entry;
+  if (p.sinks.list) {
+    if (p.sinks.joins_entries) {  // the entry of a sequence's first share stands for the sequence
+      const int2 e = p.sinks.list[entry];
+      if (e.y != 0) return;
+      seq = e.x;
+    }
+    if (seq >= pr.batch || !has_parts(p, seq)) return;
+  }
   const int column = 4 * (threadIdx.x % kQuads);
   const SeqInfo s = seq_info(pr, seq);
   const int c = n_block * kBlockN + r;
   if (n_block * kBlockN >= pr.sink || c >= s.lk || column >= p.head_dim) return;
-  const int64_t q0 = pr.cu_q ? s.q0 : (int64_t)seq * pr.seqlen_q, slot0 = q0 / p.sinks.rows + seq;
   const int shares = ceil_div(s.lq, p.sinks.rows);
   const int64_t tile = (int64_t)kBlockN * D, stride = (int64_t)pr.heads_kv * p.sinks.blocks * 2 * tile;
-  const float* part = p.sinks.part + slot0 * stride + (((int64_t)kv_head * p.sinks.blocks + n_block) * 2) * tile + r * D + column;
+  const float* part = p.sinks.part + sink_slot(p, s, seq) * stride + (((int64_t)kv_head * p.sinks.blocks + n_block) * 2) * tile + r * D + column;
   float4 dv = make_float4(0.f, 0.f, 0.f, 0.f), dk = dv;
 #pragma unroll 4
   for (int i = 0; i < shares; ++i) {
@@ -902,22 +910,26 @@ static void mark(int index, cudaStream_t stream) {
 struct BwdWorkspace {
   size_t lse_log2, dpsum, pivot_sum, pivot_key, dq_accum, dk_fix, dk_fix_bytes, work_list, sink_list, sink_part, total;
   int64_t rows, key_rows, entries;
-  int sink_rows, sink_blocks;     // SinkShares::rows and blocks
-  int64_t sink_entries;           // packed: entries of the shares' work list
+  int sink_rows, sink_least, sink_blocks;  // SinkShares::rows, least and blocks
+  int64_t sink_entries;                    // packed: entries of the shares' work list
 };
+
+// Query blocks that see an ordinary key block, and the least that is worth a share.
+static int64_t sink_window_blocks(const b200fa_problem& p) { return ((int64_t)p.window_left + p.window_right + kBlockN) / kBlockM + 1; }
+static int64_t sink_least_blocks(int64_t window_blocks) { return window_blocks > 4 ? window_blocks : 4; }
 
 // Query rows per share of the key blocks that hold sinks; 0: these blocks are not dealt out. A share should weigh about as
 // much as an ordinary key block (the window's query blocks), at most an eighth of what an SM has to do on average, so that
 // the launch ends evenly, and at least four query blocks, because a CTA has about two iterations' worth of set-up. Sinks that
 // fill more than four key blocks, windows without a right bound (whose key blocks are seen by half of the rows on average)
-// and sequences of less than two shares gain nothing.
+// and sequences of less than two shares gain nothing; in a packed batch such sequences are told apart on the device.
 static int sink_share_rows(const b200fa_problem& p, int sink) {
   if (sink <= 0 || sink > 4 * kBlockN || p.window_right < 0 || p.window_left < 0 || p.batch <= 0) return 0;
   const bool packed = p.cu_seqlens_q != nullptr;
   const int64_t row_blocks = ((packed ? 1 : (int64_t)p.batch) * p.seqlen_q + kBlockM - 1) / kBlockM;  // of all sequences
-  const int64_t window_blocks = ((int64_t)p.window_left + p.window_right + kBlockN) / kBlockM + 1;
+  const int64_t window_blocks = sink_window_blocks(p);
   const int64_t average = p.heads_kv * row_blocks * (window_blocks + ceil_div(sink, kBlockN)) / 148;
-  int64_t blocks = window_blocks > 4 ? window_blocks : 4;
+  int64_t blocks = sink_least_blocks(window_blocks);
   if (blocks < average / 8) blocks = average / 8;
   // Here, because the search below takes as many steps: a bound of 2^30 keys, meant as none, took it up to 267 ms a call.
   if (blocks * 2 * kBlockM > (int64_t)p.seqlen_q) return 0;  // (packed: no sequence can have two shares)
@@ -961,14 +973,18 @@ static BwdWorkspace plan_workspace(const b200fa_problem& p, int sink) {
   w.total = w.work_list + (size_t)w.entries * 8;
   w.sink_rows = sink_share_rows(p, sink);
   w.sink_blocks = w.sink_rows ? ceil_div(sink, kBlockN) : 0;
-  w.sink_entries = 0;
+  w.sink_entries = w.sink_least = 0;
   w.sink_list = w.sink_part = w.total;
   if (w.sink_rows) {
-    w.sink_entries = packed ? work_list_entries(p.seqlen_q, p.batch, w.sink_rows) : 0;
+    const int64_t slots = packed ? 2 * w.rows / w.sink_rows : (int64_t)p.batch * ceil_div(p.seqlen_q, w.sink_rows);
+    if (packed) {
+      w.sink_least = (int)(sink_least_blocks(sink_window_blocks(p)) * kBlockM);
+      const int64_t sequences = w.rows / w.sink_least;  // that have shares, at most
+      w.sink_entries = w.rows / w.sink_rows + (sequences < p.batch ? sequences : p.batch);
+    }
     w.sink_list = (w.total + 255) & ~size_t(255);
     w.sink_part = (w.sink_list + (size_t)w.sink_entries * 8 + 255) & ~size_t(255);
-    const size_t slots = (size_t)(w.rows / w.sink_rows) + p.batch;
-    w.total = w.sink_part + slots * p.heads_kv * w.sink_blocks * 2 * kBlockN * compiled_dim * 4;
+    w.total = w.sink_part + (size_t)slots * p.heads_kv * w.sink_blocks * 2 * kBlockN * compiled_dim * 4;
   }
   return w;
 }
@@ -1090,7 +1106,7 @@ static int launch_bwd_d(const b200fa_bwd_args& a, int sink, cudaStream_t stream)
                a.dk_stride[2] % 16 == 0 && a.dv_stride[1] % 16 == 0 && a.dv_stride[2] % 16 == 0 && bp.head_dim % 16 == 0;
   p.work_list = nullptr;
   p.n_blocks = p.head_slots = p.section = 1;
-  p.sinks = SinkShares{w.sink_rows, w.sink_blocks, 0, 0, nullptr, reinterpret_cast<float*>(ws + w.sink_part)};
+  p.sinks = SinkShares{w.sink_rows, w.sink_least, w.sink_blocks, 0, 0, false, nullptr, reinterpret_cast<float*>(ws + w.sink_part)};
   p.status = device_status_word();
   if (!p.status) return B200FA_ERR_CUDA;
   p.trace = trace_buffer();
@@ -1105,12 +1121,13 @@ static int launch_bwd_d(const b200fa_bwd_args& a, int sink, cudaStream_t stream)
   if (run_main && packed) {
     const int32_t* other = bp.cu_visible_q ? bp.cu_visible_q : bp.cu_seqlens_q;
     WorkLists lists{{bp.cu_seqlens_k, bp.cu_seqlens_q}, {other, bp.cu_seqlens_q}, {kBlockN, p.sinks.rows}, {0, 0},
-                    {(int)w.entries, (int)w.sink_entries},
+                    {(int)w.entries, (int)w.sink_entries}, {0, p.sinks.least},
                     {reinterpret_cast<int2*>(ws + w.work_list), reinterpret_cast<int2*>(ws + w.sink_list)}};
     const int status = launch_work_lists(lists, p.sinks.rows ? 2 : 1, bp.batch, stream);
     if (status != B200FA_OK) return status;
     p.work_list = reinterpret_cast<const int2*>(ws + w.work_list);
     if (p.sinks.rows) {
+      p.sinks.joins_entries = w.sink_entries < bp.batch;
       p.sinks.list = reinterpret_cast<const int2*>(ws + w.sink_list);
       p.sinks.ctas = (int)w.sink_entries * p.sinks.blocks;
     }
@@ -1180,7 +1197,8 @@ static int launch_bwd_d(const b200fa_bwd_args& a, int sink, cudaStream_t stream)
     }
     const int row_blocks = (int)post.x;
     const bool join = run_main && p.sinks.rows > 0;
-    if (join) post.x += (unsigned)(bp.batch * p.sinks.blocks * (kBlockN * D / 4 / 256));
+    const int64_t joined = p.sinks.joins_entries ? w.sink_entries : bp.batch;
+    if (join) post.x += (unsigned)(joined * p.sinks.blocks * (kBlockN * D / 4 / 256));
     auto* kernel = join ? &bwd_postprocess_kernel<D, true> : &bwd_postprocess_kernel<D, false>;
     kernel<<<post, 256, 0, stream>>>(dq_accum, map, bp.softmax_scale, static_cast<__nv_bfloat16*>(a.dq),
                                      packed ? 0 : a.dq_stride[0], a.dq_stride[1], a.dq_stride[2], fix, row_blocks, p);

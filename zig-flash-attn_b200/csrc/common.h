@@ -43,11 +43,11 @@ int encode_tensor_map(CUtensorMap* map, const void* base, CUtensorMapDataType ty
 
 Problem to_problem(const b200fa_problem& in);
 
-// Work lists of a packed batch (b200fa_work_list), up to two in one launch.
+// Work lists of a packed batch (b200fa_work_list), up to two in one launch. Sequences of at most `least` rows are left out.
 struct WorkLists {
   const int32_t* cu[2];
   const int32_t* cu_other[2];
-  int block_rows[2], descending[2], num_entries[2];
+  int block_rows[2], descending[2], num_entries[2], least[2];
   int2* table[2];
 };
 int launch_work_lists(const WorkLists& lists, int count, int batch, cudaStream_t stream);

@@ -21,7 +21,7 @@ __global__ void __launch_bounds__(kListThreads, 1) work_list_kernel(const __grid
   const int32_t* __restrict__ cu = lists.cu[blockIdx.x];
   const int32_t* __restrict__ cu_other = lists.cu_other[blockIdx.x];
   const int block_rows = lists.block_rows[blockIdx.x], descending = lists.descending[blockIdx.x];
-  const int num_entries = lists.num_entries[blockIdx.x];
+  const int num_entries = lists.num_entries[blockIdx.x], least = lists.least[blockIdx.x];
   int2* __restrict__ table = lists.table[blockIdx.x];
   __shared__ uint32_t keys[kListThreads];
   __shared__ int order[kListThreads];
@@ -39,7 +39,8 @@ __global__ void __launch_bounds__(kListThreads, 1) work_list_kernel(const __grid
       key = kClasses - 1 - length_class(other);
       // A prefix-sum array that is not non-decreasing describes no batch; its negative lengths count as empty
       // sequences, so that no entry index can become negative (the kernels that read the list then skip them).
-      blocks = ceil_div(imax(cu[i + 1] - cu[i], 0), block_rows);
+      const int rows = cu[i + 1] - cu[i];
+      blocks = rows > least ? ceil_div(rows, block_rows) : 0;
     }
     keys[tid] = key;
     __syncthreads();
