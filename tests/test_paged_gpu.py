@@ -491,3 +491,26 @@ def test_writes_raise_the_version_of_the_caches():
             out.sum().backward()
         with torch.inference_mode():
             write(randn(4, 16, 2, 64), randn(4, 16, 2, 64))
+
+
+@pytest.mark.parametrize("d, heads, lengths, page_size", [(128, (8, 2), [40, 300, 20000, 9], 16), (64, (4, 4), [40, 300, 9], 7),
+                                                         (256, (4, 2), [2000, 5, 9], 16), (512, (2, 1), [30, 5, 9], 16)])
+def test_decode_reports_what_is_no_number(d, heads, lengths, page_size):
+    """A NaN among the queries or the visible keys makes that head's output and log-sum-exp NaN, not "sees no key" (-inf)."""
+    torch.manual_seed(d)
+    table, pages = scattered(lengths, page_size)
+    k, v = randn(pages, page_size, heads[1], d), randn(pages, page_size, heads[1], d)
+    q = randn(len(lengths), heads[0], d)
+    want, want_lse, tolerance, lse_tolerance = plain.decode(q, k, v, table, lengths, d**-0.5, -1, 0)
+    group = heads[0] // heads[1]
+    bad = torch.zeros(len(lengths), heads[0], dtype=torch.bool)
+    bad[0, 0] = bad[1, :group] = True
+    for value in (float("nan"), float("inf")):
+        bad_q, bad_k = q.clone(), k.clone()
+        bad_q[0, 0, 3] = value
+        page = table[1, lengths[1] // page_size // 2]
+        bad_k[page, 1, 0, 5], bad_k[page, 2, 0, 5] = value, -value  # seen by the first key head's queries of sequence 1
+        out, lse = (x.cpu() for x in zigfa.flash_attn_paged_func(bad_q, bad_k, v, table, ints(lengths), return_attn_probs=True))
+        assert torch.isnan(out[bad]).all() and torch.isnan(lse[bad]).all()
+        assert ((out.double() - want).abs() <= tolerance)[~bad].all()  # nobody else's
+        assert ((lse.double() - want_lse).abs() <= lse_tolerance)[~bad].all()

@@ -79,12 +79,13 @@ __device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
 }
 __device__ __forceinline__ uint32_t word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
 
-// Four columns of an output row from their sums, and the row's log-sum-exp.
+// Four columns of an output row from their sums, and the row's log-sum-exp. `total` is 0 where no key is seen; a NaN among the
+// scores, or an infinite one, makes it NaN, and the row with it.
 __device__ __forceinline__ void store_output(const PagedParams& p, int b, int head, int d, float4 sum, float top, float total) {
-  const float inv = total > 0.f ? 1.f / total : 0.f;
+  const float inv = total == 0.f ? 0.f : 1.f / total;
   *reinterpret_cast<uint2*>(p.out + b * p.out_seq + head * p.out_head + d) =
       make_uint2(pack_bf16x2(sum.x * inv, sum.y * inv), pack_bf16x2(sum.z * inv, sum.w * inv));
-  if (d == 0) p.lse[(int64_t)b * p.heads_q + head] = total > 0.f ? (top + log2f(total)) * 0.69314718055994531f : -INFINITY;
+  if (d == 0) p.lse[(int64_t)b * p.heads_q + head] = total == 0.f ? -INFINITY : (top + log2f(total)) * 0.69314718055994531f;
 }
 
 // ---------------------------------------------------------------------------------------------- dealing out the steps
