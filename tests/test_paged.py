@@ -264,7 +264,7 @@ def test_the_short_way_counts_the_versions_too(monkeypatch):
     class Plain(torch.Tensor):
         is_cuda = True
 
-    monkeypatch.setattr(dispatch, "_PLAIN", (Plain, torch.Tensor))
+    monkeypatch.setattr(dispatch, "_PLAIN", {Plain, torch.Tensor})
     x, y = torch.zeros(3).as_subclass(Plain), torch.zeros(3)
     before = y._version
     probe(x, y)
@@ -273,3 +273,43 @@ def test_the_short_way_counts_the_versions_too(monkeypatch):
         frozen = torch.zeros(3)
         probe(torch.zeros(3).as_subclass(Plain), frozen)
     assert calls == [1, 1]
+
+
+def test_the_short_way_is_for_plain_arguments_only(monkeypatch):
+    """The implementations take addresses. A subclass in any place, or a transform around the call, goes to the dispatcher;
+    a subclass that wraps other tensors has the address 0."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    from zigfa._impl import dispatch
+
+    direct, wrapped = [], []
+    probe = dispatch.define("short_way_probe(Tensor x, Tensor? y, int n) -> Tensor", lambda x, y, n: direct.append(1) or x.clone(),
+                            lambda x, *unused: torch.empty_like(x))
+
+    class Cuda(torch.Tensor):  # stands for a plain tensor on a device, whose implementation may be called
+        is_cuda = True
+
+    class Wrapper(torch.Tensor):
+        @staticmethod
+        def __new__(cls, inner):
+            return torch.Tensor._make_wrapper_subclass(cls, inner.shape, dtype=inner.dtype)
+
+        def __init__(self, inner):
+            self.inner = inner
+
+        @classmethod
+        def __torch_dispatch__(cls, function, types, arguments=(), options=None):
+            wrapped.append(str(function))
+            return torch.zeros(3)
+
+    monkeypatch.setattr(dispatch, "_PLAIN", {*dispatch._PLAIN, Cuda})
+    x = torch.zeros(3).as_subclass(Cuda)
+    probe(x, None, 1)
+    probe(x, torch.zeros(3), 1)
+    assert len(direct) == 2
+    with torch._C.DisableTorchFunctionSubclass():
+        probe(x, Wrapper(torch.zeros(3)), 1)
+        assert wrapped == ["zigfa.short_way_probe.default"]
+        with pytest.raises(NotImplementedError, match="short_way_probe"):  # no kernel for the CPU behind the dispatcher
+            torch.vmap(lambda y: probe(x, y, 1))(torch.zeros(2, 3))
+    assert len(direct) == 2

@@ -514,3 +514,19 @@ def test_decode_reports_what_is_no_number(d, heads, lengths, page_size):
         assert torch.isnan(out[bad]).all() and torch.isnan(lse[bad]).all()
         assert ((out.double() - want).abs() <= tolerance)[~bad].all()  # nobody else's
         assert ((lse.double() - want_lse).abs() <= lse_tolerance)[~bad].all()
+
+
+def test_vmap_takes_the_dispatcher():
+    torch.manual_seed(16)
+    table, lengths = ints([[0, 1], [2, 3]]), ints([20, 7])
+    q, k, v = randn(3, 2, 4, 64), randn(4, 16, 2, 64), randn(4, 16, 2, 64)
+    want = torch.stack([zigfa.flash_attn_paged_func(x, k, v, table, lengths) for x in q])
+    assert torch.equal(torch.vmap(lambda x: zigfa.flash_attn_paged_func(x, k, v, table, lengths))(q), want)
+    rows = randn(3, 2, 1, 2, 64)
+    before = k.clone()
+    with pytest.raises(RuntimeError, match="append_kv|vmap|[Bb]atch"):
+        torch.vmap(lambda x: zigfa.append_paged_kv(x, x, k, v, table, lengths))(rows)
+    assert torch.equal(k, before)
+    q, k, v = randn(3, 1, 40, 2, 64), randn(1, 40, 2, 64), randn(1, 40, 2, 64)
+    want = torch.stack([zigfa.flash_attn_sink_func(x, k, v, 4, causal=True, window_size=(9, -1)) for x in q])
+    assert torch.equal(torch.vmap(lambda x: zigfa.flash_attn_sink_func(x, k, v, 4, causal=True, window_size=(9, -1)))(q), want)

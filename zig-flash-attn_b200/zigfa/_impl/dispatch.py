@@ -18,9 +18,10 @@ from torch.autograd.graph import increment_version
 from . import lib as _lib
 
 _library = torch.library.Library("zigfa", "FRAGMENT")
-_PLAIN = (torch.Tensor, torch.nn.Parameter)
+_PLAIN = {torch.Tensor, torch.nn.Parameter, type(None), int, float}
 _is_compiling = torch.compiler.is_compiling
 _modes = torch._C._len_torch_dispatch_stack
+_transform = torch._C._functorch.peek_interpreter_stack  # the innermost of torch.vmap, torch.func.grad, ...; None outside
 
 PROBLEM = "8if7P"  # b200fa_problem
 PACK_FWD = struct.Struct(f"@{PROBLEM}5P14qPN").pack
@@ -49,8 +50,11 @@ def define(schema, implementation, fake, written=()):
 
     @functools.wraps(implementation)
     def call(*arguments):
-        first = arguments[0]
-        if type(first) in _PLAIN and first.is_cuda and not _is_compiling() and not _modes():
+        # Every argument counts: the implementation takes addresses, which a tensor subclass or a batch of tensors lacks.
+        if (
+            _PLAIN.issuperset(map(type, arguments)) and arguments[0].is_cuda and not _is_compiling() and not _modes()
+            and _transform() is None
+        ):
             result = implementation(*arguments)
             for position, _ in written:
                 if not arguments[position].is_inference():  # those have no version counter

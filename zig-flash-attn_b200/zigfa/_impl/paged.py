@@ -341,6 +341,9 @@ def flash_attn_paged(q, k_cache, v_cache, block_table, cache_seqlens, softmax_sc
     if not (type(left) is int and type(right) is int and -1 <= left < 2**31 and right >= -1):
         ops.require_window(left, right)
         left = min(int(left), 2**31 - 1)
+    if type(sink_size) is not int:
+        ops.check_sink_size(sink_size)
+        sink_size = int(sink_size)
     refuse_gradients("paged attention", q, k_cache, v_cache)
     softmax_scale = ops.default_softmax_scale(softmax_scale, q.shape[-1])
     result = paged_forward(q, k_cache, v_cache, block_table, cache_seqlens, softmax_scale, left, sink_size)
