@@ -190,8 +190,8 @@ int b200fa_sink_query_blocks_host(const b200fa_problem* problem, int32_t sink_si
 /* ---- Paged key-value cache (no counterpart in the reference).
  * A cache tensor is (num_pages, page_size, heads_kv, head_dim) BF16; key j of sequence b is row j % page_size of page
  * block_table[b][j / page_size]. A table entry outside [0, num_pages) holds no page: its positions are not visible, and
- * nothing is written there. Lengths outside [0, max_pages * page_size] are cut to that range. The integer tensors are
- * int32 with contiguous columns. */
+ * nothing is written there. Lengths outside [0, max_pages * page_size] are cut to that range, except for b200fa_append_kv,
+ * where a length only says where the new tokens go. The integer tensors are int32 with contiguous columns. */
 
 /* Attention of one new token per sequence over the cache: out = softmax(scale q k^T) v over the keys that the token, the
  * last of the cache_seqlens[b] keys of its sequence, sees: the last window_left + 1 of them (-1 = all) and the first
@@ -229,7 +229,8 @@ typedef struct b200fa_kv_cache {
   int64_t k_stride[3], v_stride[3]; /* [0] page, [1] row, [2] head */
 } b200fa_kv_cache;
 
-/* Writes the keys and values of new tokens into the pages: token i of sequence b becomes key cache_seqlens[b] + i.
+/* Writes the keys and values of new tokens into the pages: token i of sequence b becomes key cache_seqlens[b] + i, and is
+ * dropped where that lies outside [0, max_pages * page_size) or on no page.
  * Fixed length: k, v (batch, rows, heads_kv, head_dim), cu_seqlens NULL. Packed: k, v (rows, heads_kv, head_dim),
  * cu_seqlens (batch + 1); rows behind the last sequence are left out. No two sequences may write to the same page. */
 typedef struct b200fa_append_args {
