@@ -313,3 +313,17 @@ def test_the_short_way_is_for_plain_arguments_only(monkeypatch):
         with pytest.raises(NotImplementedError, match="short_way_probe"):  # no kernel for the CPU behind the dispatcher
             torch.vmap(lambda y: probe(x, y, 1))(torch.zeros(2, 3))
     assert len(direct) == 2
+
+
+@pytest.mark.parametrize("d, heads_kv, batch, keys, whole", [
+    (128, 8, 1, 512, True), (128, 8, 1, 528, False), (128, 8, 16, 1280, True), (128, 8, 16, 1296, False), (64, 8, 37, 1536, True), (128, 8, 37, 1552, False), (128, 8, 24, 1296, False),
+    (128, 8, 38, 512, True), (128, 8, 38, 528, False),  # 304 pairs: a second round for eight of them
+    (128, 8, 56, 1280, True), (128, 8, 74, 1280, True), (64, 8, 76, 528, False), (128, 8, 100, 1280, True), (128, 8, 74, 1296, False),
+    (256, 4, 2, 256, True), (256, 4, 2, 272, False), (256, 4, 32, 512, True), (256, 4, 32, 528, False), (256, 4, 76, 272, False),
+    (256, 4, 148, 512, False), (512, 2, 64, 512, True), (512, 2, 80, 272, False)])
+def test_which_pairs_of_sequence_and_key_head_are_cut(d, heads_kv, batch, keys, whole):
+    args = lib.PagedArgs(batch=batch, heads_q=4 * heads_kv, heads_kv=heads_kv, head_dim=d, page_size=16, max_pages=keys // 16, window_left=-1)
+    assert (lib.library().b200fa_paged_decode_workspace_bytes(args) == 0) == whole
+    if whole:  # a window bounds the pairs whatever the table holds
+        args.max_pages, args.window_left, args.sink_size = 4096, keys // 2 - 16, keys // 2 - 32
+        assert lib.library().b200fa_paged_decode_workspace_bytes(args) == 0

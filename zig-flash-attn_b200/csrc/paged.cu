@@ -570,19 +570,32 @@ struct PagedShape {
   size_t total() const { return o_bytes + ml_bytes + cut_bytes; }
 };
 // Pairs of at most so many steps are not cut: up to there the plan and the join kernel take longer than the steps of one
-// block: 3 to 5 us on the GPU, 4 on the host. One sequence, 32/8 heads of 128 (8 pairs): 256 keys 6.3 us uncut and 9.1
-// cut, 512 keys 9.1 and 8.9, 1024 keys 13.6 and 9.4. With so many pairs that most SMs have one, longer ones need no cut
-// either: 128 pairs of 1024 keys 16.5 and 21.7, of 0 to 1500 keys 19.9 and 22.2, of 0 to 2048 keys 25.0 and 24.6.
-static int uncut_steps(int head_dim, int64_t pairs) { return (head_dim <= 128 ? 32 : 16) * (pairs >= 100 ? 3 : 1); }
+// block. A pair more than the block slots takes a whole round of its own, so longer pairs stay whole only in one round of 100
+// pairs or more, and up to head_dim 128 also in several whose last one leaves a quarter of all slots empty at most. Times in
+// us whole / cut, pages of 16 in a cache larger than L2, all sequences at the limit or of random lengths up to it:
+//   head_dim 128, 8 key heads x 4: 8 pairs of 512 keys 8.9 / 8.8, of 768 10.9 / 6.8; 128 pairs of 1280 keys 17.1 / 18.0 and
+//   15.8 / 18.6, of 1536 19.0 / 19.4 and 18.0 / 17.1; 240 of 1536 23.8 / 27.3 and 21.8 / 22.5; 304 of 1024 32.0 / 25.4 and
+//   18.2 / 23.7, of 512 20.3 / 19.1 and 15.7 / 19.6; 448 of 1280 39.1 / 38.6 and 35.3 / 32.4; 592 of 1280 40.0 / 41.7 and
+//   37.0 / 35.8. head_dim 64: 128 of 1280 13.3 / 14.9 and 11.9 / 14.9.
+//   head_dim 256, 4 x 4: 8 pairs of 256 keys 10.6 / 10.8, of 384 12.9 / 8.2; 128 of 512 17.3 / 17.9 and 17.2 / 18.2, of 768
+//   23.0 / 20.4 and 23.1 / 19.4; 304 of 512 38.2 / 27.9 and 29.9 / 28.2, of 256 23.1 / 19.5 and 23.0 / 22.8.
+//   head_dim 512, 2 x 4: 16 of 256 18.0 / 16.4 and 14.4 / 21.9; 128 of 512 30.1 / 33.7 and 30.7 / 34.8.
+static int uncut_steps(int head_dim, int64_t pairs, int slots) {
+  const int64_t rounds = (pairs + slots - 1) / slots;
+  const bool one_round = pairs >= 100 && pairs <= slots;
+  if (head_dim > 128) return one_round ? 32 : 16;
+  if (one_round) return 3 * pairs >= 2 * slots ? 96 : 80;
+  return rounds > 1 && 4 * pairs >= 3 * rounds * slots ? 80 : 32;
+}
 static PagedShape paged_shape(const b200fa_paged_args& a) {
   PagedShape s;
   const int group = a.heads_q / a.heads_kv;
   s.tiles = paged_tiles(a.head_dim, group);
   s.chunks = (group + 8 * s.tiles - 1) / (8 * s.tiles);
   const int64_t most_steps = ((int64_t)a.max_pages * a.page_size + kPagedStep - 1) / kPagedStep;
-  const int blocks_per_sm = a.head_dim <= 256 ? 2 : 1;
+  const int slots = (a.head_dim <= 256 ? 2 : 1) * kPagedSms;  // blocks that run at the same time
   const int64_t most_work = most_steps * a.batch * a.heads_kv * s.chunks, wanted = (most_work + kMinSteps - 1) / kMinSteps;
-  s.ranges = wanted < blocks_per_sm * kPagedSms ? (int)wanted : blocks_per_sm * kPagedSms;
+  s.ranges = wanted < slots ? (int)wanted : slots;
   s.o_bytes = s.ml_bytes = s.cut_bytes = 0;
   const int64_t pairs = (int64_t)a.batch * a.heads_kv * s.chunks;
   // steps of a pair, at most: a window bounds them whatever the table holds
@@ -591,13 +604,13 @@ static PagedShape paged_shape(const b200fa_paged_args& a) {
     const int64_t seen = ((int64_t)a.window_left + kPagedStep) / kPagedStep + 1 + ((int64_t)a.sink_size + kPagedStep - 1) / kPagedStep;
     pair_steps = seen < most_steps ? seen : most_steps;
   }
-  if (pair_steps <= uncut_steps(a.head_dim, pairs)) {
-    s.ranges = pairs < blocks_per_sm * kPagedSms ? (int)pairs : blocks_per_sm * kPagedSms;
+  if (pair_steps <= uncut_steps(a.head_dim, pairs, slots)) {
+    s.ranges = pairs < slots ? (int)pairs : slots;
     return s;
   }
-  const size_t slots = 2 * (size_t)s.ranges * 8 * s.tiles;
-  s.o_bytes = slots * a.head_dim * 4;
-  s.ml_bytes = slots * 8;
+  const size_t part_rows = 2 * (size_t)s.ranges * 8 * s.tiles;
+  s.o_bytes = part_rows * a.head_dim * 4;
+  s.ml_bytes = part_rows * 8;
   s.cut_bytes = (size_t)s.ranges * 16;
   return s;
 }
