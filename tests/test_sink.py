@@ -203,3 +203,15 @@ def test_workspace_of_a_packed_backward_pass_does_not_grow_with_the_number_of_do
     for documents in (2, 100, 1000, 4096):
         # the list of shares holds 8 bytes per sequence of more than `least` rows, 512 or more; both lists are aligned to 256
         assert abs(parts(documents)[0] - extra) <= 8 * (tokens // 512) + 512, documents
+
+
+def test_the_plan_counts_both_halves_of_the_head_dimension():
+    """At head_dim 256 a key block is two CTAs' work, so a share may be twice as large as with half the columns: the parts of
+    a long batch take the same memory per key head (twice the width, half the shares)."""
+    library = lib.library()
+
+    def parts(d):
+        p = problem(131072, 131072, 1023, 0, heads_q=16, heads_kv=8, head_dim=d)
+        return library.b200fa_sink_bwd_workspace_bytes(ctypes.byref(p), 4) - library.b200fa_bwd_workspace_bytes(ctypes.byref(p))
+
+    assert 0 < parts(256) <= 1.1 * parts(128)

@@ -919,16 +919,17 @@ static int64_t sink_window_blocks(const b200fa_problem& p) { return ((int64_t)p.
 static int64_t sink_least_blocks(int64_t window_blocks) { return window_blocks > 4 ? window_blocks : 4; }
 
 // Query rows per share of the key blocks that hold sinks; 0: these blocks are not dealt out. A share should weigh about as
-// much as an ordinary key block (the window's query blocks), at most an eighth of what an SM has to do on average, so that
-// the launch ends evenly, and at least four query blocks, because a CTA has about two iterations' worth of set-up. Sinks that
-// fill more than four key blocks, windows without a right bound (whose key blocks are seen by half of the rows on average)
-// and sequences of less than two shares gain nothing; in a packed batch such sequences are told apart on the device.
+// much as an ordinary key block (the window's query blocks), but not less than an eighth of what an SM has to do on average:
+// the shares start first, so finer ones end the launch no more evenly and only add parts; and not less than four query blocks,
+// because a CTA has about two iterations' worth of set-up. Sinks that fill more than four key blocks, windows without a right
+// bound (whose key blocks are seen by half of the rows on average) and sequences of less than two shares gain nothing; in a
+// packed batch such sequences are told apart on the device.
 static int sink_share_rows(const b200fa_problem& p, int sink) {
   if (sink <= 0 || sink > 4 * kBlockN || p.window_right < 0 || p.window_left < 0 || p.batch <= 0) return 0;
   const bool packed = p.cu_seqlens_q != nullptr;
   const int64_t row_blocks = ((packed ? 1 : (int64_t)p.batch) * p.seqlen_q + kBlockM - 1) / kBlockM;  // of all sequences
   const int64_t window_blocks = sink_window_blocks(p);
-  const int64_t average = p.heads_kv * row_blocks * (window_blocks + ceil_div(sink, kBlockN)) / 148;
+  const int64_t average = p.heads_kv * (p.head_dim > 128 ? 2 : 1) * row_blocks * (window_blocks + ceil_div(sink, kBlockN)) / 148;
   int64_t blocks = sink_least_blocks(window_blocks);
   if (blocks < average / 8) blocks = average / 8;
   // Here, because the search below takes as many steps: a bound of 2^30 keys, meant as none, took it up to 267 ms a call.
