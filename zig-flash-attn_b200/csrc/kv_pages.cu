@@ -20,7 +20,7 @@ struct CacheView {
   uint8_t* k;
   uint8_t* v;
   int64_t k_page, k_row, k_head, v_page, v_row, v_head;  // strides in bytes
-  int num_pages, page_size, heads;
+  int num_pages, page_size;
   FastDiv chunks, row_chunks;  // 16-byte pieces of a row of a head, and of all heads
 };
 
@@ -430,7 +430,7 @@ static int cache_view(const b200fa_kv_cache& c, CacheView* view) {
   view->v = static_cast<uint8_t*>(c.v_cache);
   view->k_page = 2 * c.k_stride[0], view->k_row = 2 * c.k_stride[1], view->k_head = 2 * c.k_stride[2];
   view->v_page = 2 * c.v_stride[0], view->v_row = 2 * c.v_stride[1], view->v_head = 2 * c.v_stride[2];
-  view->num_pages = c.num_pages, view->page_size = c.page_size, view->heads = c.heads_kv;
+  view->num_pages = c.num_pages, view->page_size = c.page_size;
   view->chunks = FastDiv::make((uint32_t)c.head_dim / 8), view->row_chunks = FastDiv::make((uint32_t)(c.heads_kv * (c.head_dim / 8)));
   return B200FA_OK;
 }

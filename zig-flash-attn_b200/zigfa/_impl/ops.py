@@ -218,7 +218,7 @@ def launch_backward(
             _lib.check(library.b200fa_bwd(ctypes.byref(args), _stream(q.device)))
 
 
-def forward_impl(q, k, v, cu_seqlens_q, cu_seqlens_k, softmax_scale, left, right, interseq=None, direction=FORWARD, sink=0):
+def forward_impl(q, k, v, cu_seqlens_q, cu_seqlens_k, softmax_scale, left, right, interseq=None, direction=FORWARD):
     check_inputs(q, k, v, cu_seqlens_q, cu_seqlens_k, direction)
     require_window(left, right)
     q, k, v = (readable(tensor) for tensor in (q, k, v))
@@ -227,14 +227,13 @@ def forward_impl(q, k, v, cu_seqlens_q, cu_seqlens_k, softmax_scale, left, right
     softmax_lse = q.new_empty(lse_shape(q, packed), dtype=torch.float32)
     launch_forward(
         q, k, v, out, softmax_lse, _contiguous_int(cu_seqlens_q), _contiguous_int(cu_seqlens_k), softmax_scale, left,
-        right, interseq, sink,
+        right, interseq,
     )
     return out, softmax_lse
 
 
 def backward_into(
-    dout, q, k, v, out, softmax_lse, cu_seqlens_q, cu_seqlens_k, softmax_scale, left, right, dq, dk, dv, interseq=None,
-    sink=0,
+    dout, q, k, v, out, softmax_lse, cu_seqlens_q, cu_seqlens_k, softmax_scale, left, right, dq, dk, dv, interseq=None
 ):
     packed = cu_seqlens_q is not None
     check_inputs(q, k, v, cu_seqlens_q, cu_seqlens_k, BACKWARD)
@@ -246,7 +245,7 @@ def backward_into(
     buffers = tuple(writable(tensor) for tensor in targets)
     launch_backward(
         dout, q, k, v, out, softmax_lse, *buffers, _contiguous_int(cu_seqlens_q), _contiguous_int(cu_seqlens_k),
-        softmax_scale, left, right, interseq, sink,
+        softmax_scale, left, right, interseq,
     )
     for target, buffer in zip(targets, buffers):
         if buffer is not target:
