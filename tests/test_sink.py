@@ -215,3 +215,12 @@ def test_the_plan_counts_both_halves_of_the_head_dimension():
         return library.b200fa_sink_bwd_workspace_bytes(ctypes.byref(p), 4) - library.b200fa_bwd_workspace_bytes(ctypes.byref(p))
 
     assert 0 < parts(256) <= 1.1 * parts(128)
+
+
+def test_results_without_rows_may_have_any_strides():
+    library = lib.library()
+    empty = problem(0, 0, 10, 0, batch=0, cu_seqlens_q=8, cu_seqlens_k=8)  # torch: a (heads, 0) tensor has the strides (1, 1)
+    args = lib.FwdArgs(problem=empty, out_stride=lib.Stride3(8, 8, 8), lse_stride=lib.Stride2(0, 1))
+    assert library.b200fa_sink_fwd_all_rows(ctypes.byref(args), 4, None) == 0
+    args = lib.BwdArgs(problem=empty, dq_stride=lib.Stride3(8, 8, 8), dk_stride=lib.Stride3(8, 8, 8), dv_stride=lib.Stride3(8, 8, 8))
+    assert library.b200fa_sink_bwd_all_rows(ctypes.byref(args), 4, None) == 0

@@ -329,3 +329,17 @@ def test_many_short_documents_next_to_long_ones(heads, d, left, sink):
         for name, (value, tolerance) in want.items():
             plain.assert_within(name, got[name][keys if name in ("dk", "dv") else rows], value, tolerance, (d, lq, lk))
         row_q, row_k = row_q + lq, row_k + lk
+
+
+@pytest.mark.parametrize("d", [64, 128, 256, 512])
+@pytest.mark.parametrize("sink, window", [(4, (3, 0)), (0, (-1, -1))])
+def test_packed_batches_of_no_rows(d, sink, window):
+    for total_q, total_k, cu_q, cu_k in ((0, 5, [0, 0], [0, 5]), (5, 0, [0, 5], [0, 0]), (0, 0, [0], [0]), (0, 0, [0, 0, 0], [0, 0, 0]),
+                                         (6, 7, [0, 3, 3], [2, 2, 7])):
+        q, k, v = (randn(n, h, d, requires_grad=d < 512) for n, h in ((total_q, 4), (total_k, 2), (total_k, 2)))
+        out, lse = zigfa.flash_attn_varlen_sink_func(q, k, v, ints(cu_q), ints(cu_k), 9, 9, sink, window_size=window, return_attn_probs=True)
+        assert out.shape == q.shape and lse.shape == (4, total_q)
+        assert (out == 0).all() and (lse == float("-inf")).all()  # no row sees a key
+        if d < 512:
+            for gradient, x in zip(torch.autograd.grad(out, (q, k, v), torch.ones_like(out)), (q, k, v)):
+                assert gradient.shape == x.shape and (gradient == 0).all()

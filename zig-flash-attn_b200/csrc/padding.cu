@@ -54,7 +54,8 @@ static int launch_clear_padding(const Padding& a, cudaStream_t stream) {
 
 // Adds a result of the pass; its rows must lie one behind the other.
 static int add(Padding* a, void* out, const int64_t* stride, const int32_t* cu, int64_t rows, int heads, int head_dim) {
-  B200FA_REQUIRE(stride[2] == head_dim && stride[1] == (int64_t)heads * head_dim, "results of all rows must be contiguous");
+  // a tensor without rows may have any strides
+  B200FA_REQUIRE(rows == 0 || (stride[2] == head_dim && stride[1] == (int64_t)heads * head_dim), "results of all rows must be contiguous");
   B200FA_REQUIRE((out || rows == 0) && head_dim % 8 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0,
                  "results of all rows need a 16-byte aligned pointer and rows of whole 16-byte pieces");
   const int i = a->count++;
@@ -75,8 +76,8 @@ int b200fa_sink_fwd_all_rows(const b200fa_fwd_args* args, int32_t sink_size, voi
     const b200fa_problem& p = args->problem;
     const int status = add(&a, args->out, args->out_stride, p.cu_seqlens_q, p.seqlen_q, p.heads_q, p.head_dim);
     if (status != B200FA_OK) return status;
-    B200FA_REQUIRE(args->lse_stride[1] == p.seqlen_q, "results of all rows must be contiguous");
-    B200FA_REQUIRE(args->softmax_lse || p.seqlen_q == 0, "null tensor pointer");
+    B200FA_REQUIRE(p.seqlen_q == 0 || args->lse_stride[1] == p.seqlen_q, "results of all rows must be contiguous");
+    B200FA_REQUIRE(p.seqlen_q == 0 || args->softmax_lse, "null tensor pointer");
     a.batch = p.batch, a.heads = p.heads_q, a.lse = args->softmax_lse;
   }
   const int status = b200fa_sink_fwd(args, sink_size, stream);
