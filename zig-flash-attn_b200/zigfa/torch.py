@@ -167,7 +167,9 @@ def append_paged_kv(
 
     k, v (sequences, tokens, heads_kv, head_dim), or packed (total, heads_kv, head_dim) with cu_seqlens (sequences + 1);
     token i of sequence b becomes key cache_seqlens[b] + i, so cache_seqlens counts the keys held before the call. Tokens
-    whose position lies outside the table, in front of key 0 included, or whose entry holds no page are dropped. Sequences must not share the pages that are written to."""
+    whose position lies outside the table, in front of key 0 included, or whose entry holds no page are dropped. Sequences must
+    not share the pages that are written to. The version counters of the caches go up: a backward pass that has saved one of
+    them raises."""
     from ._impl import paged
 
     paged.append_paged_kv(k, v, k_cache, v_cache, block_table, cache_seqlens, cu_seqlens)
